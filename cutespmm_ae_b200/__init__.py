@@ -88,6 +88,17 @@ def _load() -> C.CDLL:
                                                 C.c_uint64, C.c_uint32, vp]),
         "cutespmm_plan_device_status": (C.c_int, [vp, u32p]),
         "cutespmm_sddmm": (C.c_int, [vp, vp, C.c_uint64, vp, C.c_uint64, C.c_uint32, C.c_int, vp, vp]),
+        "cutespmm_embedding": (C.c_int, [C.c_int, vp, C.c_uint64, C.c_uint64, C.c_uint32, vp, C.c_int, C.c_uint64, C.c_float, vp, C.c_uint64, vp]),
+        "cutespmm_embedding_grad_workspace": (C.c_uint64, [C.c_uint64, C.c_uint64, C.c_uint32]),
+        "cutespmm_embedding_grad": (C.c_int, [C.c_int, vp, C.c_uint64, vp, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_float, vp, C.c_uint64, vp,
+                                              C.c_uint64, vp]),
+        "cutespmm_block_means": (C.c_int, [C.c_int, vp, vp, vp, *[C.c_uint32] * 5, vp, vp]),
+        "cutespmm_block_scores": (C.c_int, [C.c_int, vp, vp, vp, vp, *[C.c_uint32] * 6, vp, vp]),
+        "cutespmm_select_blocks": (C.c_int, [vp, vp, vp, *[C.c_uint32] * 9, vp, vp]),
+        "cutespmm_block_attention": (C.c_int, [vp, vp, vp, vp]),
+        "cutespmm_block_attention_grad_workspace": (C.c_uint64, [vp]),
+        "cutespmm_block_attention_grad": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_uint64, vp]),
+        "cutespmm_pattern_status": (C.c_int, [u32p]),
         "cutespmm_comm_unique_id": (C.c_int, [vp]),
         "cutespmm_comm_create": (C.c_int, [C.POINTER(vp), C.c_int, C.c_int, vp]),
         "cutespmm_comm_create_all": (C.c_int, [C.POINTER(vp), C.c_int, C.POINTER(C.c_int)]),

@@ -17,7 +17,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIBDIR = HERE / "lib"
 LIB = LIBDIR / "libcutespmm.so"
-SOURCES = ["capi.cu", "rows_kernel.cu", "block_rows_kernel.cu", "brick_kernel.cu", "noalloc.cu", "slab_kernel.cu", "device_build.cu", "device_plan.cu", "sharded.cu", "sddmm_kernel.cu", "plan_io.cu", "plan.cpp", "brick_build.cpp", "slab_build.cpp", "mtx_io.cpp"]
+SOURCES = ["capi.cu", "rows_kernel.cu", "block_rows_kernel.cu", "brick_kernel.cu", "noalloc.cu", "slab_kernel.cu", "device_build.cu", "device_plan.cu", "sharded.cu", "sddmm_kernel.cu", "plan_io.cu",
+           "embedding.cu", "block_select.cu", "block_attention.cu", "block_attention_grad.cu", "pattern_capi.cu", "plan.cpp", "brick_build.cpp", "slab_build.cpp", "mtx_io.cpp"]
 def _find_nvcc() -> str:
     import shutil
 
@@ -33,13 +34,14 @@ FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC,-fopenmp,-O3,-Wall,-Wno-unknown-pragmas",
-    "-shared", "-lgomp", "-ldl",
+    "-shared", "-lgomp", "-ldl", "--threads", "0",
 ]
 
 
 # The binding on torch tensors (needs torch's headers and libraries; the C ABI library needs neither).
 BIND = LIBDIR / "_torch_bind.so"
-BIND_SOURCE = CSRC / "torch_bind.cpp"
+BIND_SOURCES = [CSRC / "torch_bind.cpp", CSRC / "torch_pattern.cpp"]
+BIND_FILES = [*BIND_SOURCES, CSRC / "torch_common.hpp"]
 
 
 def _sources():
@@ -48,7 +50,7 @@ def _sources():
 
 def _stamp() -> str:
     h = hashlib.sha256()
-    for f in sorted([f for f in CSRC.glob("*") if f != BIND_SOURCE] + [HERE.parent / "include" / "cutespmm.h"]):
+    for f in sorted([f for f in CSRC.glob("*") if f not in BIND_FILES] + [HERE.parent / "include" / "cutespmm.h"]):
         if f.is_file():
             h.update(f.name.encode())
             h.update(f.read_bytes())
@@ -86,7 +88,7 @@ def _bind_stamp() -> str:
     import importlib.metadata
 
     h = hashlib.sha256(importlib.metadata.version("torch").encode())
-    for f in (BIND_SOURCE, HERE.parent / "include" / "cutespmm.h"):
+    for f in (*BIND_FILES, HERE.parent / "include" / "cutespmm.h"):
         h.update(f.read_bytes())
     return h.hexdigest()
 
@@ -112,7 +114,7 @@ def build_bind(force: bool = False) -> Path:
     include = [troot / "include", troot / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], CUDA_HOME / "include"]
     part = LIBDIR / f"{BIND.name}.{os.getpid()}"  # whole before it bears the name: other processes may be loading it
     # libstdc++ by its shared name: a static copy would not unwind the exceptions torch's libraries throw
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-isystem{d}" for d in include], "-o", str(part), str(BIND_SOURCE),
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-isystem{d}" for d in include], "-o", str(part), *map(str, BIND_SOURCES),
            f"-L{LIBDIR}", f"-L{troot / 'lib'}", "-l:" + LIB.name, "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

@@ -1,0 +1,789 @@
+// Gradients of attention over selected blocks.  With P = exp(scale q K^T - lse), D = dout V^T and delta = <dout, out> per row:
+//   dS = P (D - delta),   dq = scale dS K,   dk = scale dS^T q,   dv = P^T dout.
+//
+// Two walks over the pattern, each with sums of its own and in a fixed order, so nothing is added by atomics:
+//   * dq by tiles of neighbouring queries over the union of their blocks, like the forward kernel (block_attention_dq_kernel);
+//   * dk and dv by tiles of 64 keys over the queries that name them (block_attention_dkv_kernel).  That needs the pattern turned round:
+//     a bit per (block, query), from which the kernel reads a tile's queries in ascending order.
+// P is formed again in each of the two from lse; nothing of size queries x keys is stored.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "block_attention.cuh"
+#include "device_plan.hpp"
+#include "num.cuh"
+#include "pattern_ops.hpp"
+#include "ptx.cuh"
+#include "tc16.cuh"
+
+namespace cutespmm {
+namespace {
+
+__device__ uint32_t g_status;  // set to 1 (dq) or 2 (dk, dv) when a bounded wait gives up
+
+// ---- dq ----------------------------------------------------------------------------------------------------------------
+// The forward kernel's tile and ring; a warp has one tile of eight columns, with q, dout and dq of it in registers, and takes a unit 16
+// keys at a time.  A masked key's dS is zero whatever K and V hold there, and its K is cut out of the product with dS.
+constexpr int kDqWarps = 8;
+constexpr int kDqRingBytes = 64 * 1024;
+template <int DP, int UNIT> constexpr int kDqHalf = DP / 64 * UNIT * 128;
+template <int DP, int UNIT> constexpr int kDqUnit = 2 * kDqHalf<DP, UNIT>;
+template <int DP, int UNIT> constexpr int kDqRing = kDqRingBytes / kDqUnit<DP, UNIT> < 8 ? kDqRingBytes / kDqUnit<DP, UNIT> : 8;
+
+template <class T, int DP, int UNIT>
+__global__ void __launch_bounds__((kDqWarps + 1) * 32, 2) block_attention_dq_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttentionArgs a, uint32_t stride, uint32_t tile_queries, uint32_t chunks)
+{
+    constexpr int STAGES = kDqRing<DP, UNIT>, DT = DP / 16;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * kDqUnit<DP, UNIT>), *empty = full + STAGES;
+    volatile uint32_t *gave_up = reinterpret_cast<volatile uint32_t *>(empty + STAGES);
+    BlockUnion u(reinterpret_cast<unsigned char *>(empty + STAGES + 2), tile_queries, a.count, a.num_blocks);
+    const uint32_t t0 = blockIdx.x * tile_queries, b = blockIdx.z;
+    const uint32_t kv = blockIdx.y / chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % chunks * kHeadChunk;
+    const uint32_t heads = min(kHeadChunk, group - head0), queries = min(tile_queries, a.queries - t0);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], kDqWarps);
+        }
+        *gave_up = 0;
+        ptx::fence_mbar_init();
+    }
+    ptx::grid_wait();
+    ptx::grid_release();
+    u.build(a, b, kv, t0, queries);
+    const uint32_t per_block = a.block / UNIT, units = *u.size * per_block;
+
+    if (warp == kDqWarps) {
+        if (lane == 0) {
+            uint32_t i = 0;
+            for (; i < units && !*gave_up; ++i) {
+                const uint32_t s = i % STAGES;
+                if (!ptx::mbar_wait(&empty[s], ((i / STAGES) & 1u) ^ 1u)) {
+                    *gave_up = 1;
+                    break;
+                }
+                int row, outer;
+                unit_place(a, b, u.blocks[i / per_block], i % per_block * UNIT, row, outer);
+                unsigned char *stage = smem + s * kDqUnit<DP, UNIT>;
+                ptx::mbar_expect_tx(&full[s], kDqUnit<DP, UNIT>);
+#pragma unroll
+                for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + h * UNIT * 128, &k_map, h * 64, (int)kv, row, outer, &full[s]);
+#pragma unroll
+                for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + kDqHalf<DP, UNIT> + h * UNIT * 128, &v_map, h * 64, (int)kv, row, outer, &full[s]);
+            }
+            if (*gave_up) {
+                atomicExch(&g_status, 1u);
+                for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j) ptx::mbar_wait(&full[j % STAGES], (j / STAGES) & 1u);
+            }
+        }
+        return;
+    }
+
+    const uint32_t c0 = warp * 8;
+    const uint32_t c = c0 + lane / 4, ct = c / stride, ch = c % stride;
+    const bool row_on = ct < queries && ch < heads;
+    const uint64_t out_row = ((uint64_t)b * a.queries + t0 + ct) * a.heads + kv * group + head0 + ch;
+    uint32_t q[DT][2], g[DT][2];
+    float delta = 0.f;
+    {
+        const T *qr = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(t0 + ct) * a.q_query + (int64_t)(kv * group + head0 + ch) * a.q_head;
+        const T *gr = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(t0 + ct) * a.do_query + (int64_t)(kv * group + head0 + ch) * a.do_head;
+        const T *orow = static_cast<const T *>(a.out) + out_row * a.dim;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t at = d * 16 + h * 8 + 2 * (lane & 3);
+                const bool on = row_on && at < a.dim;
+                q[d][h] = on ? *reinterpret_cast<const uint32_t *>(qr + at) : 0u;
+                g[d][h] = on ? *reinterpret_cast<const uint32_t *>(gr + at) : 0u;
+                if (on) delta += to_f32(gr[at]) * to_f32(orow[at]) + to_f32(gr[at + 1]) * to_f32(orow[at + 1]);
+            }
+    }
+    delta += __shfl_xor_sync(~0u, delta, 1);
+    delta += __shfl_xor_sync(~0u, delta, 2);
+    const uint64_t stat = ((uint64_t)b * a.heads + kv * group + head0 + ch) * a.queries + t0 + ct;
+    float lse = row_on ? a.lse[stat] : 0.f;
+    if (row_on && (lane & 3) == 0) a.delta[stat] = delta;
+    uint32_t asks = 0;
+    for (uint32_t j = c0 / stride; j <= (c0 + 7) / stride; ++j)
+        if (j < queries && c0 - min(c0, j * stride) < heads) asks |= 1u << j;
+    // the statistics of the two columns this lane holds of a product
+    uint32_t query[2];
+    int sees[2];
+    float base[2], dl[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t from = (2 * (lane & 3) + h) * 4, t = __shfl_sync(~0u, ct, from);
+        const bool on = __shfl_sync(~0u, (int)row_on, from);
+        base[h] = __shfl_sync(~0u, lse, from) * kLog2e;
+        dl[h] = __shfl_sync(~0u, delta, from);
+        query[h] = on ? t : 32u;
+        sees[h] = on ? (int)u.visible[t] : 0;
+    }
+    float dq[DT][4];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.f;
+    const float scale_log2 = a.scale * kLog2e;
+
+    for (uint32_t n = 0; n < units; ++n) {
+        const uint32_t s = n % STAGES, slot = n / per_block, names = u.names[slot];
+        const int first = (int)(u.blocks[slot] * a.block + n % per_block * UNIT);
+        if (!ptx::mbar_wait(&full[s], (n / STAGES) & 1u)) {
+            *gave_up = 1;
+            if (lane == 0) atomicExch(&g_status, 1u);
+            return;
+        }
+        if (names & asks) {
+            const uint32_t keys = ptx::smem_u32(smem + s * kDqUnit<DP, UNIT>), values = keys + kDqHalf<DP, UNIT>;
+            int limit[2];
+            bool whole = true;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                limit[h] = query[h] < 32u && ((names >> query[h]) & 1u) ? sees[h] - first : 0;
+                whole = whole && (query[h] == 32u || limit[h] >= UNIT);
+            }
+            whole = __all_sync(~0u, whole);
+#pragma unroll
+            for (int k = 0; k < UNIT / 16; ++k) {
+                float sc[4] = {0.f, 0.f, 0.f, 0.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const uint32_t at = (d >> 2) * UNIT * 128 + tc::swizzled(k * 16 + (lane & 15), (d & 3) * 2 + (lane >> 4));
+                    uint32_t f[4];
+                    tc::ldmatrix4(f, keys + at);
+                    tc::mma16<T>(sc, f, q[d][0], q[d][1]);
+                    tc::ldmatrix4(f, values + at);
+                    tc::mma16<T>(dp, f, g[d][0], g[d][1]);
+                }
+                float ds[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int h = j & 1, row = k * 16 + (int)(lane >> 2) + (j >> 1) * 8;
+                    const float p = tc::exp2_fast(fmaf(sc[j], scale_log2, -base[h]));
+                    ds[j] = row < limit[h] ? p * (dp[j] - dl[h]) : 0.f;
+                }
+                const uint32_t b0 = tc::transpose8x8(tc::round2<T>(ds[0], ds[1])), b1 = tc::transpose8x8(tc::round2<T>(ds[2], ds[3]));
+                auto k_frag = [&](uint32_t (&f)[4], int d) {
+                    tc::ldmatrix4_trans(f, keys + (d >> 2) * UNIT * 128 + tc::swizzled(k * 16 + ((lane >> 4) << 3) + (lane & 7), (d & 3) * 2 + ((lane >> 3) & 1)));
+                };
+                if (whole) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        uint32_t f[4];
+                        k_frag(f, d);
+                        tc::mma16<T>(dq[d], f, b0, b1);
+                    }
+                } else {  // a pass per query whose part of the unit differs, as in the forward kernel
+                    uint32_t left = names & asks;
+                    bool all = true;
+                    while (left) {
+                        int cut = UNIT;
+                        uint32_t taken = 0;
+                        if (all) {
+                            for (uint32_t m = left; m; m &= m - 1) {
+                                const uint32_t t = __ffs(m) - 1;
+                                if ((int)u.visible[t] - first >= UNIT) taken |= 1u << t;
+                            }
+                            all = false;
+                        } else {
+                            const uint32_t t = __ffs(left) - 1;
+                            taken = 1u << t;
+                            cut = (int)u.visible[t] - first;
+                        }
+                        left &= ~taken;
+                        if (!taken || cut <= k * 16) continue;
+                        const bool mine0 = query[0] < 32u && ((taken >> query[0]) & 1u), mine1 = query[1] < 32u && ((taken >> query[1]) & 1u);
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            float o[4] = {dq[d][0], dq[d][1], dq[d][2], dq[d][3]};
+                            uint32_t f[4];
+                            k_frag(f, d);
+                            if (cut < UNIT) {
+                                const int at = k * 16 + 2 * (int)(lane & 3);
+                                f[0] = keep_keys(f[0], at, cut);
+                                f[1] = keep_keys(f[1], at, cut);
+                                f[2] = keep_keys(f[2], at + 8, cut);
+                                f[3] = keep_keys(f[3], at + 8, cut);
+                            }
+                            tc::mma16<T>(o, f, b0, b1);
+                            if (mine0) {
+                                dq[d][0] = o[0];
+                                dq[d][2] = o[2];
+                            }
+                            if (mine1) {
+                                dq[d][1] = o[1];
+                                dq[d][3] = o[3];
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&empty[s]);
+    }
+    T *row = static_cast<T *>(a.dq) + out_row * a.dim;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        const uint32_t lo = tc::transpose8x8(tc::round2<T>(dq[d][0] * a.scale, dq[d][1] * a.scale));
+        const uint32_t hi = tc::transpose8x8(tc::round2<T>(dq[d][2] * a.scale, dq[d][3] * a.scale));
+        const uint32_t at = d * 16 + 2 * (lane & 3);
+        if (row_on && at < a.dim) *reinterpret_cast<uint32_t *>(row + at) = lo;
+        if (row_on && at + 8 < a.dim) *reinterpret_cast<uint32_t *>(row + at + 8) = hi;
+    }
+}
+
+// ---- the pattern turned round ------------------------------------------------------------------------------------------
+constexpr uint32_t kKeyTile = 64;      // keys of a tile of dk and dv
+constexpr uint32_t kItemRows = 4096;   // (query, head) rows that one work item takes at least, unless the tile has fewer
+
+// Where the parts of the workspace begin (bytes), and the sizes they follow from.
+struct GradLayout {
+    uint32_t words, tiles;  // words of a block's bits over the queries; key tiles of a sequence
+    uint64_t tile_rows;     // key tiles of all sequences and heads of keys
+    uint32_t item_queries;  // queries of a work item
+    uint64_t max_items, max_slots;
+    uint64_t delta, bits, bits_bytes, counts, items, totals, partial, total;
+    explicit GradLayout(const AttentionArgs &a)
+    {
+        const uint32_t group = a.heads / a.kv_heads;
+        words = (a.queries + 31) / 32;
+        tiles = (a.keys + kKeyTile - 1) / kKeyTile;
+        tile_rows = (uint64_t)a.batch * a.kv_heads * tiles;
+        // every pair of a query and a block it names is in one tile, in two where a block is two tiles
+        const uint64_t pairs = (uint64_t)a.batch * a.kv_heads * a.queries * a.count * (a.block > kKeyTile ? 2 : 1);
+        uint64_t rows = pairs * group / 4096;  // about 4096 items in large jobs
+        if (rows < kItemRows) rows = kItemRows;
+        item_queries = (uint32_t)(rows / group < a.queries ? rows / group : a.queries);
+        if (item_queries == 0) item_queries = 1;
+        max_items = pairs / item_queries + tile_rows;
+        max_slots = 2 * (pairs / item_queries) + 1;  // a tile with two items or more has more than half of them full
+        uint64_t at = 0;
+        auto take = [&](uint64_t bytes) { const uint64_t p = at; at += (bytes + 255) / 256 * 256; return p; };
+        delta = take((uint64_t)a.batch * a.heads * a.queries * 4);
+        bits_bytes = (uint64_t)a.batch * a.kv_heads * a.num_blocks * words * 4;
+        bits = take(bits_bytes);
+        counts = take(tile_rows * 12);  // queries, then the first item, then the first slot of each tile
+        items = take(max_items * 8);
+        totals = take(8);
+        partial = take(max_slots * 2 * kKeyTile * (a.dim <= 64 ? 64 : 128) * 4);
+        total = at;
+    }
+};
+
+struct TurnArgs {
+    AttentionArgs a;
+    uint32_t words, tiles, item_queries;
+    uint64_t tile_rows;
+    uint32_t *bits, *counts, *first_item, *first_slot;
+    uint2 *items;      // (tile row, which of its items)
+    uint32_t *totals;  // items
+    float *partial;
+};
+
+// A warp per 32 queries: lane i sets query i's bit in the blocks it names.
+__global__ void __launch_bounds__(256) pattern_bits_kernel(TurnArgs p)
+{
+    ptx::grid_wait();
+    ptx::grid_release();
+    const AttentionArgs &a = p.a;
+    const uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint32_t lane = threadIdx.x & 31;
+    if (w >= (uint64_t)a.batch * a.kv_heads * p.words) return;
+    const uint32_t word = (uint32_t)(w % p.words), bh = (uint32_t)(w / p.words), b = bh / a.kv_heads, t = word * 32 + lane;
+    if (t >= a.queries) return;
+    const uint32_t visible = visible_keys(a, b, t);
+    const int32_t *src = a.blocks + ((uint64_t)bh * a.queries + t) * a.count;
+    for (uint32_t i = 0; i < a.count; ++i) {
+        const int32_t j = src[i];
+        if (block_counts(a, b, j, visible)) atomicOr(p.bits + ((uint64_t)bh * a.num_blocks + j) * p.words + word, 1u << lane);
+    }
+}
+
+// The queries that name some block of a key tile, 32 of them.
+__device__ __forceinline__ uint32_t tile_word(const TurnArgs &p, uint64_t tile_row, uint32_t word)
+{
+    const AttentionArgs &a = p.a;
+    const uint32_t tile = (uint32_t)(tile_row % p.tiles);
+    const uint64_t bh = tile_row / p.tiles;
+    const uint32_t b0 = tile * kKeyTile / a.block, b1 = min((tile * kKeyTile + kKeyTile - 1) / a.block, a.num_blocks - 1);
+    uint32_t any = 0;
+    for (uint32_t j = b0; j <= b1; ++j) any |= p.bits[(bh * a.num_blocks + j) * p.words + word];
+    return any;
+}
+
+__global__ void __launch_bounds__(256) pattern_count_kernel(TurnArgs p)
+{
+    ptx::grid_wait();
+    ptx::grid_release();
+    const uint64_t row = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= p.tile_rows) return;
+    uint32_t n = 0;
+    for (uint32_t w = threadIdx.x & 31; w < p.words; w += 32) n += __popc(tile_word(p, row, w));
+    n = __reduce_add_sync(~0u, n);
+    if ((threadIdx.x & 31) == 0) p.counts[row] = n;
+}
+
+// One block: the work items of every tile, in order; slots for partial sums where a tile has several.
+__global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
+{
+    __shared__ uint2 warp_sum[32];
+    ptx::grid_wait();
+    ptx::grid_release();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t items_before = 0, slots_before = 0;
+    for (uint64_t r0 = 0; r0 < p.tile_rows; r0 += 1024) {
+        const uint64_t row = r0 + threadIdx.x;
+        const uint32_t n = row < p.tile_rows ? (p.counts[row] + p.item_queries - 1) / p.item_queries : 0u, slots = n > 1 ? n : 0u;
+        uint32_t si = n, ss = slots;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t ui = __shfl_up_sync(~0u, si, d), us = __shfl_up_sync(~0u, ss, d);
+            if (lane >= (uint32_t)d) {
+                si += ui;
+                ss += us;
+            }
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = make_uint2(si, ss);
+        __syncthreads();
+        uint32_t bi = items_before + si - n, bs = slots_before + ss - slots;
+        for (uint32_t w = 0; w < 32; ++w) {
+            if (w < warp) {
+                bi += warp_sum[w].x;
+                bs += warp_sum[w].y;
+            }
+            items_before += warp_sum[w].x;
+            slots_before += warp_sum[w].y;
+        }
+        if (row < p.tile_rows) {
+            p.first_item[row] = bi;
+            p.first_slot[row] = bs;
+            for (uint32_t i = 0; i < n; ++i) p.items[bi + i] = make_uint2((uint32_t)row, i);
+        }
+    }
+    if (threadIdx.x == 0) p.totals[0] = items_before;
+}
+
+// ---- dk and dv ---------------------------------------------------------------------------------------------------------
+// One thread block per SM walks work items: 64 keys and a range of the queries that name them.  The queries' rows of q and dout (all heads of
+// the group: a TMA box each) are gathered into tiles of 128 rows; per tile
+//     S  = Q K^T   and  D = dO V^T       (128 x 64 each, tensor memory, two buffers)
+//     P, dS in registers of eight warps (thread = row: lse, delta and the limit of the row are one value each), written as 16-bit operands
+//     dV^T += dO^T P  and  dK^T += Q^T dS  (dims x 64 keys, accumulators in tensor memory for the whole item)
+// with the same shared-memory bytes of Q and dO serving as row-major operand of the first pair and as transposed operand of the second.
+// The tile after is multiplied while this one's P and dS are formed.  Every query names its keys by choice, so no row of a tile is
+// wasted, however little neighbouring queries agree; this is what makes the 128-row instruction the right one here.
+constexpr int kDkvWarps = 8;  // softmax warps; warp 8 loads, warp 9 multiplies
+constexpr int kDkvThreads = (kDkvWarps + 2) * 32;
+constexpr int kDkvStages = 2;
+constexpr uint32_t kTmemS = 0, kTmemD = 64, kTmemBuffer = 128, kTmemDv = 256, kTmemDk = 320, kTmemCols = 512;
+
+template <int DP> struct DkvSmem {
+    static constexpr int kHalves = DP / 64;
+    static constexpr int kKeys = 0;                                     // 64 rows x 128 bytes per 64 dims
+    static constexpr int kValues = kKeys + kHalves * 64 * 128;
+    static constexpr int kTileBytes = kHalves * 128 * 128;              // 128 rows of q (or dout)
+    static constexpr int kStage = kValues + kHalves * 64 * 128;         // per stage q, then dout
+    static constexpr int kP = kStage + kDkvStages * 2 * kTileBytes;     // 128 rows x 64 keys
+    static constexpr int kDs = kP + 128 * 128;
+    static constexpr int kLists = kDs + 128 * 128;                      // per stage the queries of a tile
+    static constexpr int kBars = kLists + kDkvStages * 128 * 4;
+    static constexpr int kBytes = kBars + 16 * 8 + 16;
+};
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kDkvThreads, 1)
+    block_attention_dkv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap do_map, TurnArgs p)
+{
+    using S = DkvSmem<DP>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const AttentionArgs &a = p.a;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars);  // q and dout of a stage have landed, its list is written
+    uint64_t *empty = full + kDkvStages;                             // the products that read the stage are done
+    uint64_t *kv_full = empty + kDkvStages;
+    uint64_t *scored = kv_full + 1;                                  // S and D of a buffer are complete (2)
+    uint64_t *formed = scored + 2;                                   // P and dS are written
+    uint64_t *used = formed + 1;                                     // the products that read P and dS are done
+    uint64_t *summed = used + 1;                                     // an item's accumulators are complete
+    uint64_t *read = summed + 1;                                     // ... and have been read
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + S::kBars + 16 * 8);  // [0] tensor memory, [1] gave up
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kDkvStages; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        ptx::mbar_init(kv_full, 1);
+        ptx::mbar_init(&scored[0], 1);
+        ptx::mbar_init(&scored[1], 1);
+        ptx::mbar_init(formed, kDkvWarps);
+        ptx::mbar_init(used, 1);
+        ptx::mbar_init(summed, 1);
+        ptx::mbar_init(read, kDkvWarps);
+        misc[1] = 0;
+        ptx::fence_mbar_init();
+    }
+    // rows of a tile behind its last query are never loaded: zeros for good
+    for (int i = threadIdx.x; i < kDkvStages * 2 * S::kTileBytes / 16; i += kDkvThreads) reinterpret_cast<uint4 *>(smem + S::kStage)[i] = make_uint4(0, 0, 0, 0);
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kTmemCols);
+    ptx::fence_async_smem();
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = misc[0];
+    ptx::grid_wait();
+    ptx::grid_release();
+
+    const uint32_t group = a.heads / a.kv_heads, per_tile = 128 / group;
+    const uint32_t items = p.totals[0];
+    uint32_t tile_count = 0;  // tiles of all items so far
+    bool ok = true;
+    auto tiles_of = [&](uint2 it) {
+        const uint32_t n = min(p.counts[it.x] - it.y * p.item_queries, p.item_queries);
+        return (n + per_tile - 1) / per_tile;
+    };
+
+    if (warp == kDkvWarps) {
+        // ================= loads =================
+        for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
+            const uint2 it = p.items[i];
+            const uint32_t tile = it.x % p.tiles, bh = it.x / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
+            const uint32_t n_tiles = tiles_of(it);
+            uint32_t left = min(p.counts[it.x] - it.y * p.item_queries, p.item_queries);
+            if (k && !(ok = ptx::mbar_wait(summed, (k - 1) & 1u))) break;
+            if (lane == 0) {
+                ptx::mbar_expect_tx(kv_full, 2 * S::kHalves * 64 * 128);
+                for (int h = 0; h < S::kHalves; ++h) {
+                    tc::tma_load4(smem + S::kKeys + h * 64 * 128, &k_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
+                    tc::tma_load4(smem + S::kValues + h * 64 * 128, &v_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
+                }
+            }
+            // a window of 32 words of the tile's bits, one per lane; the queries of earlier items are passed over
+            uint32_t skip = it.y * p.item_queries, window = 0, word = 0;
+            auto next_window = [&]() {
+                word = window + lane < p.words ? tile_word(p, it.x, window + lane) : 0u;
+                window += 32;
+            };
+            next_window();
+            for (;;) {
+                const uint32_t n = __reduce_add_sync(~0u, __popc(word));
+                if (n > skip || window >= p.words) break;
+                skip -= n;
+                next_window();
+            }
+            for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
+                const uint32_t s = tile_count % kDkvStages;
+                if (!(ok = ptx::mbar_wait(&empty[s], ((tile_count / kDkvStages) & 1u) ^ 1u))) break;
+                uint32_t *list = reinterpret_cast<uint32_t *>(smem + S::kLists) + s * 128;
+                const uint32_t want = min(per_tile, left);
+                uint32_t got = 0;
+                while (got < want) {
+                    const uint32_t mine = __popc(word);
+                    uint32_t at = mine;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const uint32_t up = __shfl_up_sync(~0u, at, d);
+                        if (lane >= (uint32_t)d) at += up;
+                    }
+                    const uint32_t n = __shfl_sync(~0u, at, 31);
+                    at -= mine;
+                    // this lane's queries have ranks at, at + 1, ... in the window; ranks below `skip` are passed over
+                    const uint32_t end = min(n, skip + want - got);
+                    for (; word && at < end; ++at) {
+                        const uint32_t bit = __ffs(word) - 1;
+                        word &= word - 1;
+                        if (at >= skip) list[got + at - skip] = (window - 32 + lane) * 32 + bit;
+                    }
+                    got += end > skip ? end - skip : 0u;
+                    skip = 0;
+                    if (got < want) {
+                        if (window >= p.words) break;  // cannot be: the counts are those of these bits
+                        next_window();
+                    }
+                }
+                for (uint32_t r = got + lane; r < per_tile; r += 32) list[r] = a.queries;  // no such query: its rows arrive as zeros
+                left -= want;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_expect_tx(&full[s], per_tile * group * 128 * S::kHalves * 2);
+                __syncwarp();
+                unsigned char *q = smem + S::kStage + s * 2 * S::kTileBytes, *g = q + S::kTileBytes;
+                for (uint32_t r = lane; r < per_tile; r += 32) {
+                    const int t = (int)list[r];
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        const uint32_t at = h * 128 * 128 + r * group * 128;
+                        tc::tma_load4(q + at, &q_map, h * 64, (int)(kv * group), t, (int)b, &full[s]);
+                        tc::tma_load4(g + at, &do_map, h * 64, (int)(kv * group), t, (int)b, &full[s]);
+                    }
+                }
+            }
+        }
+        if (!ok) {
+            misc[1] = 1;
+            if (lane == 0) {  // no copy stays in flight
+                ptx::mbar_wait(kv_full, 0);
+                ptx::mbar_wait(kv_full, 1);
+                for (uint32_t j = tile_count > kDkvStages ? tile_count - kDkvStages : 0; j < tile_count; ++j) ptx::mbar_wait(&full[j % kDkvStages], (j / kDkvStages) & 1u);
+            }
+        }
+    } else if (warp == kDkvWarps + 1) {
+        // ================= products =================
+        if (lane == 0) {
+            constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+            constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_t = tc::idesc(bf16, 128, 64, true, true);
+            const uint32_t base = ptx::smem_u32(smem);
+            // dims as rows: with 64 of them the second block of the 128-row instruction is the first once more, and its rows are left alone
+            constexpr uint32_t block_bytes = DP == 128 ? 128 * 128 : 0;
+            uint32_t done = 0;  // tiles whose second products are issued
+            auto second = [&](uint32_t k, bool first, bool last) {
+                const uint32_t s = done % kDkvStages;
+                ok = ptx::mbar_wait(formed, done & 1u) && (!first || !k || ptx::mbar_wait(read, (k - 1) & 1u));
+                if (!ok) return;
+                tc::fence_after();
+                const uint32_t q = base + S::kStage + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDv, tc::desc_mn(g + r * 2048, block_bytes), tc::desc_mn(base + S::kP + r * 2048, 0), id_t, !first || r);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDk, tc::desc_mn(q + r * 2048, block_bytes), tc::desc_mn(base + S::kDs + r * 2048, 0), id_t, !first || r);
+                tc::commit(&empty[s]);
+                tc::commit(used);
+                if (last) tc::commit(summed);
+                ++done;
+            };
+            for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
+                const uint32_t n_tiles = tiles_of(p.items[i]);
+                if (!(ok = ptx::mbar_wait(kv_full, k & 1u))) break;
+                for (uint32_t j = 0; j < n_tiles && ok; ++j, ++tile_count) {
+                    const uint32_t s = tile_count % kDkvStages, buffer = tmem + (tile_count & 1u) * kTmemBuffer;
+                    if (!(ok = ptx::mbar_wait(&full[s], (tile_count / kDkvStages) & 1u))) break;
+                    tc::fence_after();
+                    const uint32_t q = base + S::kStage + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+                        tc::mma(buffer + kTmemS, tc::desc_k(q + (d >> 2) * 128 * 128 + (d & 3) * 32), tc::desc_k(base + S::kKeys + (d >> 2) * 64 * 128 + (d & 3) * 32), id_s, d != 0);
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+                        tc::mma(buffer + kTmemD, tc::desc_k(g + (d >> 2) * 128 * 128 + (d & 3) * 32), tc::desc_k(base + S::kValues + (d >> 2) * 64 * 128 + (d & 3) * 32), id_s, d != 0);
+                    tc::commit(&scored[tile_count & 1u]);
+                    if (j) second(k, j == 1, false);
+                }
+                if (ok) second(k, n_tiles == 1, true);
+            }
+            if (!ok) misc[1] = 1;
+        }
+    } else {
+        // ================= P and dS =================
+        const uint32_t r = (warp & 3) * 32 + lane, half = warp >> 2, entry = r / group, head = r % group;
+        const float scale_log2 = a.scale * kLog2e;
+        const uint32_t lanes = tmem + (((warp & 3) * 32) << 16);
+        for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
+            const uint2 it = p.items[i];
+            const uint32_t tile = it.x % p.tiles, bh = it.x / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
+            const uint32_t n_tiles = tiles_of(it);
+            const uint32_t blocks_per_tile = a.block < kKeyTile ? kKeyTile / a.block : 1, block0 = tile * kKeyTile / a.block;
+            for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
+                const uint32_t s = tile_count % kDkvStages;
+                if (!(ok = ptx::mbar_wait(&full[s], (tile_count / kDkvStages) & 1u))) break;
+                const uint32_t t = entry < per_tile ? reinterpret_cast<const uint32_t *>(smem + S::kLists)[s * 128 + entry] : a.queries;
+                const bool on = t < a.queries;
+                float lse = 0.f, delta = 0.f;
+                int limit = 0;
+                uint32_t named = 0;  // which blocks of the tile the query names
+                if (on) {
+                    const uint64_t at = ((uint64_t)b * a.heads + kv * group + head) * a.queries + t;
+                    lse = a.lse[at] * kLog2e;
+                    delta = a.delta[at];
+                    limit = (int)visible_keys(a, b, t) - (int)(tile * kKeyTile) - (int)half * 32;
+                    if (blocks_per_tile == 1) named = 1;
+                    else
+                        for (uint32_t n = 0; n < blocks_per_tile && block0 + n < a.num_blocks; ++n)
+                            named |= ((p.bits[((uint64_t)bh * a.num_blocks + block0 + n) * p.words + (t >> 5)] >> (t & 31)) & 1u) << n;
+                }
+                // a bit per key of this thread's half
+                uint32_t sees = limit >= 32 ? ~0u : limit > 0 ? (1u << limit) - 1u : 0u;
+                if (blocks_per_tile == 2) sees = (named >> half) & 1u ? sees : 0u;
+                if (blocks_per_tile == 4) sees &= ((named >> (2 * half)) & 1u ? 0xffffu : 0u) | ((named >> (2 * half + 1)) & 1u ? 0xffff0000u : 0u);
+                const uint32_t buffer = lanes + (tile_count & 1u) * kTmemBuffer + half * 32;
+                if (!(ok = ptx::mbar_wait(&scored[tile_count & 1u], (tile_count >> 1) & 1u))) break;
+                tc::fence_after();
+                uint32_t sv[32], dv[32];
+                tc::ld32(buffer + kTmemS, sv);
+                tc::ld32(buffer + kTmemD, dv);
+                tc::wait_ld();
+                uint32_t pp[16], dd[16];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    float pv[2], ds[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool seen = (sees >> (2 * c + h)) & 1u;
+                        const float e = tc::exp2_fast(fmaf(__uint_as_float(sv[2 * c + h]), scale_log2, -lse));
+                        pv[h] = seen ? e : 0.f;
+                        ds[h] = seen ? e * (__uint_as_float(dv[2 * c + h]) - delta) : 0.f;
+                    }
+                    pp[c] = tc::round2<T>(pv[0], pv[1]);
+                    dd[c] = tc::round2<T>(ds[0], ds[1]);
+                }
+                if (tile_count && !(ok = ptx::mbar_wait(used, (tile_count - 1) & 1u))) break;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t at = tc::swizzled(r, half * 4 + c);
+                    *reinterpret_cast<uint4 *>(smem + S::kP + at) = make_uint4(pp[4 * c], pp[4 * c + 1], pp[4 * c + 2], pp[4 * c + 3]);
+                    *reinterpret_cast<uint4 *>(smem + S::kDs + at) = make_uint4(dd[4 * c], dd[4 * c + 1], dd[4 * c + 2], dd[4 * c + 3]);
+                }
+                ptx::fence_async_smem();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(formed);
+            }
+            if (!ok) break;
+            // ---- the item's sums: warps 0-3 dv, warps 4-7 dk; thread = dim ----
+            if (!(ok = ptx::mbar_wait(summed, k & 1u))) break;
+            tc::fence_after();
+            const bool is_dk = half != 0;
+            const uint32_t d = r, n_items = (p.counts[it.x] + p.item_queries - 1) / p.item_queries;
+            const float f = is_dk ? a.scale : 1.f;
+#pragma unroll 1
+            for (uint32_t c = 0; c < 64; c += 32) {
+                uint32_t v[32];
+                tc::ld32(lanes + (is_dk ? kTmemDk : kTmemDv) + c, v);
+                tc::wait_ld();
+                if (d >= a.dim) continue;
+                if (n_items == 1) {
+                    T *dst = static_cast<T *>(is_dk ? a.dk : a.dv) + (((uint64_t)b * a.keys + tile * kKeyTile + c) * a.kv_heads + kv) * a.dim + d;
+                    const uint32_t n = a.keys > tile * kKeyTile + c ? min(32u, a.keys - tile * kKeyTile - c) : 0u;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if ((uint32_t)x < n) dst[(uint64_t)x * a.kv_heads * a.dim] = from_f32<T>(f * __uint_as_float(v[x]));
+                } else {
+                    float *dst = p.partial + (((uint64_t)p.first_slot[it.x] + it.y) * 2 + (is_dk ? 1 : 0)) * kKeyTile * DP + c * DP + d;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) __stcs(dst + x * DP, f * __uint_as_float(v[x]));
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(read);
+        }
+        if (!ok) misc[1] = 1;
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && misc[1]) atomicExch(&g_status, 2u);
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tmem, kTmemCols);
+    }
+}
+
+// Key tiles that no query names are zero; the partial sums of those with several work items are added in order.
+template <class T, int DP> __global__ void __launch_bounds__(256) dkv_join_kernel(TurnArgs p)
+{
+    ptx::grid_wait();
+    ptx::grid_release();
+    const AttentionArgs &a = p.a;
+    const uint32_t row = blockIdx.x, items = (p.counts[row] + p.item_queries - 1) / p.item_queries;
+    if (items == 1) return;
+    const uint32_t tile = row % p.tiles, bh = row / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
+    const uint32_t n = min(kKeyTile, a.keys - tile * kKeyTile);
+    const float *src = p.partial + (uint64_t)p.first_slot[row] * 2 * kKeyTile * DP;
+    for (uint32_t i = threadIdx.x; i < 2 * n * (DP / 4); i += 256) {
+        const uint32_t d = i % (DP / 4) * 4, key = i / (DP / 4) % n, is_dk = i / (DP / 4) / n;
+        if (d >= a.dim) continue;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t k = 0; k < items; ++k) {
+            const float4 x = __ldcs(reinterpret_cast<const float4 *>(src + ((uint64_t)k * 2 + is_dk) * kKeyTile * DP + key * DP + d));
+            sum.x += x.x;
+            sum.y += x.y;
+            sum.z += x.z;
+            sum.w += x.w;
+        }
+        T *dst = static_cast<T *>(is_dk ? a.dk : a.dv) + (((uint64_t)b * a.keys + tile * kKeyTile + key) * a.kv_heads + kv) * a.dim + d;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(tc::round2<T>(sum.x, sum.y), tc::round2<T>(sum.z, sum.w));
+    }
+}
+
+template <class T, int DP, int UNIT> cudaError_t launch_dq(const AttentionArgs &a, cudaStream_t s)
+{
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    CUtensorMap k_map{}, v_map{};
+    if (a.keys) {
+        cudaError_t e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, UNIT);
+        if (e == cudaSuccess) e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, UNIT);
+        if (e != cudaSuccess) return e;
+    }
+    const uint32_t group = a.heads / a.kv_heads, heads = group < kHeadChunk ? group : kHeadChunk, stride = column_stride(heads), chunks = (group + kHeadChunk - 1) / kHeadChunk;
+    const uint32_t queries = kDqWarps * 8 / stride < kTileQueries ? kDqWarps * 8 / stride : kTileQueries;
+    cudaError_t e = allow_dynamic_smem<block_attention_dq_kernel<T, DP, UNIT>>(160 * 1024);
+    if (e != cudaSuccess) return e;
+    const uint32_t bytes = kDqRing<DP, UNIT> * (kDqUnit<DP, UNIT> + 16) + 16 + BlockUnion::bytes(queries, a.count, a.num_blocks);
+    const dim3 grid((a.queries + queries - 1) / queries, a.kv_heads * chunks, a.batch);
+    return launch_overlapped(block_attention_dq_kernel<T, DP, UNIT>, grid, dim3((kDqWarps + 1) * 32), bytes, s, k_map, v_map, a, stride, queries, chunks);
+}
+
+template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count, cudaStream_t s)
+{
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const GradLayout l(a);
+    char *w = static_cast<char *>(a.workspace);
+    a.delta = reinterpret_cast<float *>(w + l.delta);
+    cudaError_t e = a.block == 16 ? launch_dq<T, DP, 16>(a, s) : a.block == 32 ? launch_dq<T, DP, 32>(a, s) : launch_dq<T, DP, 64>(a, s);
+    if (e != cudaSuccess || !a.keys) return e;
+    TurnArgs p{};
+    p.a = a;
+    p.words = l.words;
+    p.tiles = l.tiles;
+    p.item_queries = l.item_queries;
+    p.tile_rows = l.tile_rows;
+    p.bits = reinterpret_cast<uint32_t *>(w + l.bits);
+    p.counts = reinterpret_cast<uint32_t *>(w + l.counts);
+    p.first_item = p.counts + l.tile_rows;
+    p.first_slot = p.first_item + l.tile_rows;
+    p.items = reinterpret_cast<uint2 *>(w + l.items);
+    p.totals = reinterpret_cast<uint32_t *>(w + l.totals);
+    p.partial = reinterpret_cast<float *>(w + l.partial);
+    if ((e = cudaMemsetAsync(p.bits, 0, l.bits_bytes, s)) != cudaSuccess) return e;
+    const uint64_t bit_warps = (uint64_t)a.batch * a.kv_heads * l.words;
+    if ((e = launch_overlapped(pattern_bits_kernel, dim3((unsigned)((bit_warps + 7) / 8)), dim3(256), 0, s, p)) != cudaSuccess) return e;
+    if ((e = launch_overlapped(pattern_count_kernel, dim3((unsigned)((l.tile_rows + 7) / 8)), dim3(256), 0, s, p)) != cudaSuccess) return e;
+    if ((e = launch_overlapped(pattern_items_kernel, dim3(1), dim3(1024), 0, s, p)) != cudaSuccess) return e;
+    CUtensorMap k_map, v_map, q_map, do_map;
+    const uint32_t group = a.heads / a.kv_heads;
+    if ((e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, kKeyTile)) != cudaSuccess) return e;
+    if ((e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, kKeyTile)) != cudaSuccess) return e;
+    if ((e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, 1, group)) != cudaSuccess) return e;
+    if ((e = tc::make_map(&do_map, bf16, a.dout, a.dim, a.heads, a.queries, a.batch, a.do_head, a.do_query, a.do_batch, 1, group)) != cudaSuccess) return e;
+    if ((e = allow_dynamic_smem<block_attention_dkv_kernel<T, DP>>(DkvSmem<DP>::kBytes)) != cudaSuccess) return e;
+    const uint64_t blocks = l.max_items < (uint64_t)sm_count ? l.max_items : (uint64_t)sm_count;
+    if ((e = launch_overlapped(block_attention_dkv_kernel<T, DP>, dim3((unsigned)blocks), dim3(kDkvThreads), DkvSmem<DP>::kBytes, s, k_map, v_map, q_map, do_map, p)) != cudaSuccess) return e;
+    return launch_overlapped(dkv_join_kernel<T, DP>, dim3((unsigned)l.tile_rows), dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+uint64_t block_attention_grad_workspace(const AttentionArgs &a) { return GradLayout(a).total; }
+
+cudaError_t launch_block_attention_grad(const AttentionArgs &a, int sm_count, cudaStream_t s)
+{
+    if (!a.batch || !a.heads || !a.dim) return cudaSuccess;
+    const uint64_t kv_bytes = (uint64_t)a.batch * a.keys * a.kv_heads * a.dim * 2;
+    if (!a.queries || !a.count) {  // nobody looks at any key
+        cudaError_t e = cudaSuccess;
+        if (kv_bytes && (e = cudaMemsetAsync(a.dk, 0, kv_bytes, s)) == cudaSuccess) e = cudaMemsetAsync(a.dv, 0, kv_bytes, s);
+        if (e == cudaSuccess && a.queries) e = cudaMemsetAsync(a.dq, 0, (uint64_t)a.batch * a.queries * a.heads * a.dim * 2, s);
+        return e;
+    }
+    if (a.dtype == CUTESPMM_BF16) return a.dim <= 64 ? launch_grad<__nv_bfloat16, 64>(a, sm_count, s) : launch_grad<__nv_bfloat16, 128>(a, sm_count, s);
+    return a.dim <= 64 ? launch_grad<__half, 64>(a, sm_count, s) : launch_grad<__half, 128>(a, sm_count, s);
+}
+
+cudaError_t block_attention_grad_status(uint32_t *word) { return read_status(g_status, word); }
+
+}  // namespace cutespmm

@@ -1,0 +1,337 @@
+// Which blocks of keys a query attends to: the mean key of every block, the score of every query against every mean, and per query
+// the blocks of the highest scores.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "device_plan.hpp"
+#include "num.cuh"
+#include "pattern_ops.hpp"
+#include "ptx.cuh"
+#include "tc16.cuh"
+
+namespace cutespmm {
+namespace {
+
+__device__ uint32_t g_status;  // set to 1 when a bounded wait of the score kernel gives up
+
+// ---- means -------------------------------------------------------------------------------------------------------------
+// A block of threads takes 32 groups of eight columns (of all heads side by side) of one block of keys: eight warps walk its rows,
+// every load is 512 contiguous bytes where the heads are.  Sums in fp32, one rounding.  Bound: HBM (the keys once).
+constexpr int kMeanWarps = 8;
+
+template <class T> __global__ void __launch_bounds__(kMeanWarps * 32) block_means_kernel(MeansArgs a)
+{
+    __shared__ float part[kMeanWarps][32][9];
+    ptx::grid_wait();
+    ptx::grid_release();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, packs = a.dim / 8;
+    const uint32_t col = blockIdx.x * 32 + lane, blk = blockIdx.y, b = blockIdx.z;
+    const uint32_t head = col / packs, d = col % packs * 8;
+    const bool on = head < a.kv_heads;
+    const uint32_t keys = a.lengths ? (uint32_t)min(max(a.lengths[b], 0), (int)a.keys) : a.keys;
+    const uint32_t first = blk * a.block, n = first < keys ? min(a.block, keys - first) : 0u;
+    const T *src = static_cast<const T *>(a.k) + (int64_t)b * a.k_batch + (int64_t)head * a.k_head + d + (int64_t)first * a.k_key;
+    float acc[8] = {};
+#pragma unroll 4
+    for (uint32_t r = warp; r < n; r += kMeanWarps)
+        if (on) {
+            const Pack<T, 8> p = load_pack<T, 8>(src + (int64_t)r * a.k_key);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += to_f32(p.x[j]);
+        }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][lane][j] = acc[j];
+    __syncthreads();
+    // thread t adds column t of the 256 over the warps
+    const uint32_t l = threadIdx.x >> 3, j = threadIdx.x & 7, out_col = blockIdx.x * 32 + l;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMeanWarps; ++w) sum += part[w][l][j];
+    if (out_col < a.kv_heads * packs)
+        static_cast<T *>(a.means)[((uint64_t)b * a.blocks + blk) * a.kv_heads * a.dim + (uint64_t)out_col * 8 + j] = from_f32<T>(n ? sum / (float)n : 0.f);
+}
+
+// ---- scores ------------------------------------------------------------------------------------------------------------
+// scores[t, n] = sum over the heads h of a group of q[t, h] . means[n]: one product with heads and dims side by side as K, so that the
+// sum over heads costs no additions of its own and q is read once.  Per block 128 queries x up to 256 means; the means stay in shared
+// memory (they are the same operand for every head), q arrives through a ring of TMA tiles, the products of 16-bit values are exact and
+// are added in fp32 in tensor memory.  Bound: HBM (q and the scores).
+constexpr int kScoreRows = 128, kScoreCols = 256, kScoreStages = 3;
+constexpr int kScoreStageBytes = kScoreRows * 128;
+constexpr int kScoreMeans = kScoreStages * kScoreStageBytes;                 // offset of the means: two tiles of 256 rows x 128 bytes
+constexpr int kScoreBars = kScoreMeans + 2 * kScoreCols * 128;
+constexpr int kScoreSmem = kScoreBars + 128;
+constexpr int kScoreThreads = 192;  // warps 0-3 read the accumulator back, warp 4 loads, warp 5 multiplies
+
+template <class T> __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap m_map, ScoresArgs a)
+{
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kScoreBars), *empty = full + kScoreStages, *means_in = empty + kScoreStages, *done = means_in + 1;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(done + 1);  // [0] tensor memory, [1] gave up
+    const uint32_t n0 = blockIdx.x * kScoreCols, t0 = blockIdx.y * kScoreRows;
+    const uint32_t b = blockIdx.z / a.kv_heads, kv = blockIdx.z % a.kv_heads, group = a.heads / a.kv_heads;
+    const uint32_t halves = (a.dim + 63) / 64, steps = group * halves;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kScoreStages; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        ptx::mbar_init(means_in, 1);
+        ptx::mbar_init(done, 1);
+        misc[1] = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kScoreCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = misc[0];
+    ptx::grid_wait();
+    ptx::grid_release();
+    if (warp == 4 && lane == 0) {
+        ptx::mbar_expect_tx(means_in, halves * kScoreCols * 128);
+        for (uint32_t h = 0; h < halves; ++h) tc::tma_load4(smem + kScoreMeans + h * kScoreCols * 128, &m_map, (int)(h * 64), (int)kv, (int)n0, (int)b, means_in);
+        for (uint32_t i = 0; i < steps; ++i) {
+            const uint32_t s = i % kScoreStages;
+            if (!ptx::mbar_wait(&empty[s], ((i / kScoreStages) & 1u) ^ 1u)) {
+                misc[1] = 1;
+                break;
+            }
+            ptx::mbar_expect_tx(&full[s], kScoreStageBytes);
+            tc::tma_load4(smem + s * kScoreStageBytes, &q_map, (int)(i % halves * 64), (int)(kv * group + i / halves), (int)t0, (int)b, &full[s]);
+        }
+    } else if (warp == 5 && lane == 0) {
+        constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, kScoreRows, kScoreCols);
+        bool ok = ptx::mbar_wait(means_in, 0);
+        for (uint32_t i = 0; i < steps && ok; ++i) {
+            const uint32_t s = i % kScoreStages;
+            if (!(ok = ptx::mbar_wait(&full[s], (i / kScoreStages) & 1u))) break;
+            tc::fence_after();
+            const uint64_t ad = tc::desc_k(ptx::smem_u32(smem + s * kScoreStageBytes)), bd = tc::desc_k(ptx::smem_u32(smem + kScoreMeans + i % halves * kScoreCols * 128));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc::mma(tmem, ad + 2 * k, bd + 2 * k, id, i || k);
+            tc::commit(&empty[s]);
+        }
+        if (!ok) misc[1] = 1;
+        tc::commit(done);
+    } else if (warp < 4) {
+        // accumulator -> rows of scores, 32 x 32 at a time through shared memory (the ring is free by then), so that a store is 128
+        // contiguous bytes of one row whatever the row's alignment
+        if (ptx::mbar_wait(done, 0)) {
+            tc::fence_after();
+            float *tile = reinterpret_cast<float *>(smem) + warp * 32 * 33;
+            float *out = a.scores + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0 + warp * 32) * a.blocks + n0;
+            const uint32_t rows = t0 + warp * 32 < a.queries ? min(32u, a.queries - t0 - warp * 32) : 0u;
+            for (uint32_t c = 0; c < kScoreCols && n0 + c < a.blocks; c += 32) {
+                uint32_t v[32];
+                tc::ld32(tmem + ((warp * 32) << 16) + c, v);
+                tc::wait_ld();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = __uint_as_float(v[j]);
+                __syncwarp();
+                if (n0 + c + lane < a.blocks)
+                    for (uint32_t r = 0; r < rows; ++r) __stcs(out + (uint64_t)r * a.blocks + c + lane, tile[r * 33 + lane]);
+            }
+        } else if (lane == 0)
+            misc[1] = 1;
+        tc::fence_before();
+    }
+    __syncthreads();
+    if (misc[1] && threadIdx.x == 0) {  // a wait gave up: report, and leave no copy in flight behind
+        atomicExch(&g_status, 1u);
+        ptx::mbar_wait(means_in, 0);
+        for (uint32_t s = 0; s < kScoreStages; ++s)
+            for (uint32_t p = 0; p < 2; ++p) ptx::mbar_wait(&full[s], p);
+    }
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tmem, kScoreCols);
+    }
+}
+
+// ---- selection ---------------------------------------------------------------------------------------------------------
+// WARPS warps take one row of scores, 32 * R consecutive ones each, in registers as unsigned integers of the same order (0: not to be
+// chosen; all ones: chosen in any case).  The count-th largest is found bit by bit from the top -- how many are at least this
+// candidate? -- and the search ends as soon as a candidate leaves exactly `count`.  Then the chosen indices are written in ascending
+// order, equal scores from the lowest index on.  Bound: HBM in large calls (the visible scores once), latency in small ones.
+template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) select_blocks_kernel(SelectArgs a, uint64_t rows)
+{
+    constexpr int kRowsPerBlock = WARPS == 1 ? 4 : 1;
+    __shared__ uint32_t counts[WARPS][2];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = WARPS == 1 ? 0 : warp;
+    ptx::grid_wait();
+    ptx::grid_release();
+    const uint64_t row = (uint64_t)blockIdx.x * kRowsPerBlock + (WARPS == 1 ? warp : 0);
+    if (row >= rows) return;
+    const uint32_t t = (uint32_t)(row % a.queries), bh = (uint32_t)(row / a.queries), b = bh / a.kv_heads;
+    const int64_t see = a.visible ? a.visible[(uint64_t)b * a.queries + t] : (int64_t)a.keys - a.queries + 1 + t;
+    const uint32_t visible = (uint32_t)min(max(see, (int64_t)0), (int64_t)a.keys);
+    const uint32_t n = min((visible + a.block - 1) / a.block, a.blocks);
+    const float *src = a.scores + (int64_t)b * a.s_batch + (int64_t)(bh % a.kv_heads) * a.s_head + (int64_t)t * a.s_query;
+    const uint32_t i0 = part * R * 32 + lane;
+    uint32_t key[R];
+    uint32_t any = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t i = i0 + r * 32;
+        key[r] = 0;
+        if (i < n) {
+            const float f = __ldg(src + i) + 0.f;  // -0 becomes 0: they are equal scores
+            const uint32_t bits = __float_as_uint(f);
+            if (f > -INFINITY) key[r] = (bits >> 31) ? ~bits : bits | 0x80000000u;  // neither NaN nor -infinity
+            if (i < a.first || i + a.last >= n) key[r] = ~0u;
+        }
+        any += key[r] != 0;
+    }
+    // how many of the row
+    auto total = [&](uint32_t v) {
+        v = __reduce_add_sync(~0u, v);
+        if constexpr (WARPS > 1) {
+            __syncthreads();
+            if (lane == 0) counts[warp][0] = v;
+            __syncthreads();
+            v = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) v += counts[w][0];
+        }
+        return v;
+    };
+    uint32_t limit = 1;     // chosen: every key above it, and the first `ties` that equal it
+    uint32_t ties = ~0u;
+    if (total(any) > a.count) {
+        limit = 0;
+        bool exact = false;
+        for (int bit = 31; bit >= 0 && !exact; --bit) {
+            const uint32_t cand = limit | (1u << bit);
+            uint32_t c = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) c += key[r] >= cand;
+            c = total(c);
+            if (c >= a.count) limit = cand;
+            exact = c == a.count;
+        }
+        if (!exact) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) c += key[r] > limit;
+            ties = a.count - total(c);
+        }
+    }
+    uint32_t before = 0, ties_before = 0;  // chosen, and equal to the limit, at lower indices
+    if constexpr (WARPS > 1) {
+        uint32_t above = 0, equal = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            above += key[r] > limit;
+            equal += key[r] == limit;
+        }
+        above = __reduce_add_sync(~0u, above);
+        equal = __reduce_add_sync(~0u, equal);
+        __syncthreads();
+        if (lane == 0) {
+            counts[warp][0] = above;
+            counts[warp][1] = equal;
+        }
+        __syncthreads();
+        for (uint32_t w = 0; w < part; ++w) {
+            before += counts[w][0];
+            ties_before += counts[w][1];
+        }
+        before += min(ties_before, ties);
+    }
+    int32_t *out = a.out + row * a.count;
+    const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t equal = __ballot_sync(~0u, key[r] == limit);
+        const bool tie = key[r] == limit && ties_before + __popc(equal & below) < ties;
+        const uint32_t chosen = __ballot_sync(~0u, key[r] > limit || tie);
+        if ((chosen >> lane) & 1u) out[before + __popc(chosen & below)] = (int32_t)(i0 + r * 32);
+        before += __popc(chosen);
+        ties_before += __popc(equal);
+    }
+    if (part == WARPS - 1)
+        for (uint32_t i = before + lane; i < a.count; i += 32) out[i] = -1;
+}
+
+}  // namespace
+
+cudaError_t launch_block_means(const MeansArgs &a, cudaStream_t s)
+{
+    if (!a.batch || !a.blocks || !a.kv_heads || !a.dim) return cudaSuccess;
+    const dim3 grid((a.kv_heads * (a.dim / 8) + 31) / 32, a.blocks, a.batch);
+    return a.dtype == CUTESPMM_BF16 ? launch_overlapped(block_means_kernel<__nv_bfloat16>, grid, dim3(kMeanWarps * 32), 0, s, a)
+                                    : launch_overlapped(block_means_kernel<__half>, grid, dim3(kMeanWarps * 32), 0, s, a);
+}
+
+cudaError_t launch_block_scores(const ScoresArgs &a, int sm_count, cudaStream_t s)
+{
+    (void)sm_count;
+    if (!a.batch || !a.queries || !a.kv_heads || !a.blocks) return cudaSuccess;
+    const bool bf16 = a.dtype == CUTESPMM_BF16;
+    CUtensorMap q_map, m_map;
+    cudaError_t e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, kScoreRows);
+    if (e == cudaSuccess) e = tc::make_map(&m_map, bf16, a.means, a.dim, a.kv_heads, a.blocks, a.batch, a.m_head, a.m_block, a.m_batch, kScoreCols);
+    if (e == cudaSuccess) e = bf16 ? allow_dynamic_smem<block_scores_kernel<__nv_bfloat16>>(kScoreSmem) : allow_dynamic_smem<block_scores_kernel<__half>>(kScoreSmem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((a.blocks + kScoreCols - 1) / kScoreCols, (a.queries + kScoreRows - 1) / kScoreRows, a.batch * a.kv_heads);
+    return bf16 ? launch_overlapped(block_scores_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a)
+                : launch_overlapped(block_scores_kernel<__half>, grid, dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a);
+}
+
+cudaError_t launch_select_blocks(const SelectArgs &a, int sm_count, cudaStream_t s)
+{
+    const uint64_t rows = (uint64_t)a.batch * a.kv_heads * a.queries;
+    if (!rows || !a.count) return cudaSuccess;
+    auto one = [&](auto kernel) { return launch_overlapped(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, a, rows); };
+    auto eight = [&](auto kernel) { return launch_overlapped(kernel, dim3((unsigned)rows), dim3(256), 0, s, a, rows); };
+    // eight warps a row where there are too few rows to fill the machine with a warp each, or too many scores for one warp's registers
+    if (a.blocks <= 1024 && (a.blocks <= 32 || rows > (uint64_t)sm_count * 8)) {
+        if (a.blocks <= 32) return one(select_blocks_kernel<1, 1>);
+        if (a.blocks <= 64) return one(select_blocks_kernel<2, 1>);
+        if (a.blocks <= 128) return one(select_blocks_kernel<4, 1>);
+        if (a.blocks <= 256) return one(select_blocks_kernel<8, 1>);
+        if (a.blocks <= 512) return one(select_blocks_kernel<16, 1>);
+        return one(select_blocks_kernel<32, 1>);
+    }
+    if (a.blocks <= 256) return eight(select_blocks_kernel<1, 8>);
+    if (a.blocks <= 1024) return eight(select_blocks_kernel<4, 8>);
+    if (a.blocks <= 4096) return eight(select_blocks_kernel<16, 8>);
+    return eight(select_blocks_kernel<64, 8>);
+}
+
+namespace tc {
+
+cudaError_t make_map(CUtensorMap *out, bool bf16, const void *p, uint32_t dim, uint32_t heads, uint32_t rows, uint32_t outer, int64_t head_stride, int64_t row_stride,
+                     int64_t outer_stride, uint32_t box_rows, uint32_t box_heads)
+{
+    using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                       CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeTiledFn enc = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    if (!enc) return cudaErrorNotSupported;
+    // the stride of an extent of one is never used, but has to be one that a map can hold
+    auto bytes = [](int64_t stride, uint32_t extent) { return (cuuint64_t)(extent > 1 ? stride * 2 : 16); };
+    const cuuint64_t dims[4] = {dim, heads, rows, outer};
+    const cuuint64_t strides[3] = {bytes(head_stride, heads), bytes(row_stride, rows), bytes(outer_stride, outer)};
+    const cuuint32_t box[4] = {64, box_heads, box_rows, 1}, one[4] = {1, 1, 1, 1};
+    return enc(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+}  // namespace tc
+
+cudaError_t block_select_status(uint32_t *word) { return read_status(g_status, word); }
+
+}  // namespace cutespmm

@@ -55,6 +55,15 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, 
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Reads a status word that is a __device__ variable of the calling file on the current device and clears it where it is set.
+template <class Symbol> cudaError_t read_status(Symbol &symbol, uint32_t *word)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(word, symbol, sizeof *word);
+    const uint32_t zero = 0;
+    if (e == cudaSuccess && *word) e = cudaMemcpyToSymbol(symbol, &zero, sizeof zero);
+    return e;
+}
+
 // Arguments of the row-gather kernel.
 struct RowsArgs {
     const uint32_t *row_ptr;   // M+1 offsets into pairs

@@ -6,14 +6,10 @@
 // (2-3 us), and the operators' forward and backward run without the interpreter.
 //
 // The plans themselves stay with the Python objects (Plan, SparseOperator); this file holds handles only.
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <ATen/ops/empty.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <c10/cuda/CUDAStream.h>
 
 #include <memory>
 #include <mutex>
@@ -21,42 +17,15 @@
 #include <string>
 #include <unordered_map>
 
-#include "../../include/cutespmm.h"
+#include "torch_common.hpp"
 
 namespace {
 
 using at::Tensor;
-
-PyObject *g_error_class = nullptr;  // CuteSpmmError(status, message)
-
-// The GIL is held.
-void set_status_error(int status)
-{
-    const char *msg = cutespmm_last_error();
-    if (!msg || !*msg) msg = cutespmm_status_string(status);
-    PyObject *e = g_error_class ? PyObject_CallFunction(g_error_class, "is", status, msg) : nullptr;
-    if (e) {
-        PyErr_SetObject(reinterpret_cast<PyObject *>(Py_TYPE(e)), e);
-        Py_DECREF(e);
-    } else if (!PyErr_Occurred()) {
-        PyErr_SetString(PyExc_RuntimeError, msg);
-    }
-}
-
-void check_status(int status)  // with or without the GIL
-{
-    if (status == CUTESPMM_OK) return;
-    PyGILState_STATE g = PyGILState_Ensure();
-    set_status_error(status);
-    python_error err;
-    err.persist();
-    PyGILState_Release(g);
-    throw err;
-}
+using namespace bind;
 
 bool dense2d(const Tensor &t) { return t.is_cuda() && t.scalar_type() == at::kFloat && t.dim() == 2 && t.stride(1) == 1; }
 uint64_t ld(const Tensor &t, int64_t rows) { return rows > 1 ? (uint64_t)t.stride(0) : (uint64_t)std::max<int64_t>(t.size(1), 1); }
-void *stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 const float *in(const Tensor &t) { return static_cast<const float *>(t.const_data_ptr()); }
 float *out(const Tensor &t) { return static_cast<float *>(t.mutable_data_ptr()); }
 Tensor new_dense(int64_t rows, int64_t cols, const Tensor &like) { return at::empty({rows, cols}, like.options().requires_grad(false)); }
@@ -186,10 +155,6 @@ Tensor op_sddmm(int64_t id, const Tensor &X, const Tensor &Y, bool scale)
     return run_sddmm(op->plan, op->M, op->K, op->nnz, unit_stride(X), unit_stride(Y), Tensor(), scale, nullptr);
 }
 
-template <class Sig> c10::TypedOperatorHandle<Sig> handle(const char *name)
-{
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
-}
 using Unary = Tensor(int64_t, const Tensor &);
 using Weighted = Tensor(int64_t, const Tensor &, const Tensor &);
 Tensor call_spmm(int64_t id, const Tensor &B)
@@ -284,40 +249,6 @@ TORCH_LIBRARY_IMPL(cutespmm, Autograd, m)
 }
 
 // ---- the Python module -----------------------------------------------------------------------------------------------
-
-const Tensor &tensor(PyObject *o, const char *what)
-{
-    TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a torch tensor");
-    return THPVariable_Unpack(o);
-}
-Tensor tensor_or_none(PyObject *o, const char *what) { return o == Py_None ? Tensor() : tensor(o, what); }
-int64_t integer(PyObject *o)
-{
-    const int64_t v = o == Py_None ? 0 : (int64_t)PyLong_AsUnsignedLongLong(o);
-    if (PyErr_Occurred()) throw python_error();
-    return v;
-}
-void *pointer(PyObject *o) { return reinterpret_cast<void *>(integer(o)); }
-void want_args(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, "expected ", want, " arguments, got ", n); }
-// a stream the caller named: its handle (the default stream's is 0, which the calls above read as "the current one")
-void *named_stream(PyObject *o)
-{
-    if (o == Py_None) return nullptr;
-    void *s = pointer(o);
-    return s ? s : reinterpret_cast<void *>(0x1);  // cudaStreamLegacy
-}
-
-// fn without the interpreter lock, as ctypes makes its calls: a launch that waits for room in its stream's queue must not hold
-// up other threads, and threads that drive a stream each run side by side.  The calls below take their arguments out of
-// Python first and hold references of their own to the tensors.
-template <class Fn> auto without_gil(Fn &&fn)
-{
-    struct Released {
-        PyThreadState *state = PyEval_SaveThread();
-        ~Released() { PyEval_RestoreThread(state); }
-    } released;
-    return fn();
-}
 
 PyObject *py_spmm(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
@@ -473,4 +404,12 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_bind", "Hot calls of cute
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_bind(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__torch_bind(void)
+{
+    PyObject *m = PyModule_Create(&g_module);
+    if (m && bind::add_pattern_calls(m) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

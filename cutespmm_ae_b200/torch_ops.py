@@ -17,10 +17,23 @@ to its values.  `op.weighted(w, B)` is the attention form (TCGNN.cpp:260-264, fo
 stored nonzero in the plan's storage order, typically normalised `op.sddmm` scores -- replaces the plan's values
 (Plan.set_values) before the product; its gradients are dB = A_w^T @ dC (the transposed plan receives w through a
 permutation computed once) and dw = sddmm(dC, B).
+
+The functions at the end of this file are products whose sparse pattern the data choose in each call, so no plan fits them.  They
+have no counterpart in the reference:
+
+    out = embedding(tokens, table, scale)                    # one-hot matrix times a table; differentiable with respect to the table
+    means = block_means(k, block)                            # mean key of every block of keys
+    scores = block_scores(q, means)                          # a cheap score of every block for every query
+    blocks = select_blocks(scores, count, block, keys)       # the blocks of the highest scores, per query
+    out = block_attention(q, k, v, blocks, block)            # attention over those; differentiable with respect to q, k and v
+
+Each is an operator `torch.ops.cutespmm.<name>` as well, runs on torch's current stream of the operands' device, and may be captured
+in a CUDA graph.  Operands whose strides or alignment a kernel cannot read are copied first.
 """
 from __future__ import annotations
 
 import itertools
+import math
 import threading
 import weakref
 
@@ -32,7 +45,8 @@ from . import _native as _load_native
 
 _native = _load_native()
 
-__all__ = ["SparseOperator", "register_plan", "unregister_plan", "transpose_csr"]
+__all__ = ["SparseOperator", "register_plan", "unregister_plan", "transpose_csr", "embedding", "block_means", "block_scores", "select_blocks",
+           "block_attention", "pattern_status"]
 
 _plans: dict[int, "SparseOperator"] = {}
 _ids = itertools.count(1)
@@ -184,3 +198,108 @@ def _(plan_id: int, w: torch.Tensor, G: torch.Tensor) -> torch.Tensor:
 @torch.library.register_fake("cutespmm::sddmm")
 def _(plan_id: int, X: torch.Tensor, Y: torch.Tensor, scale_by_values: bool) -> torch.Tensor:
     return X.new_empty((_get(plan_id).nnz,))
+
+
+# ---- products whose pattern the data choose in each call -----------------------------------------------------------
+
+
+def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[tokens], [*tokens.shape, dim], in the table's type (float32, float16, bfloat16; one rounding).  tokens: int32 or
+    int64 of any shape; one outside [0, vocab), a padded position for instance, names no row: its output is zero and it sends no gradient.
+
+    The gradient of the table is dense, [vocab, dim].  Its rows are sums over the tokens that name them, in fp32 and in the order of
+    their positions (tokens are sorted on the device in the backward pass), so it has the same bits in every run."""
+    if torch.compiler.is_compiling():
+        return torch.ops.cutespmm.embedding(tokens, table, scale)
+    return _native.op_embedding(tokens, table, scale)
+
+
+def block_means(k: torch.Tensor, block: int, lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """Mean key of every block of `block` (16, 32, 64, 128) keys: k [batch, keys, kv_heads, dim] (float16 or bfloat16, dim a multiple of 8 up
+    to 128) -> [batch, ceil(keys / block), kv_heads, dim].  The last block's mean is over the keys it has; with `lengths` (int32, [batch]) only
+    the first lengths[b] keys of a sequence count, and a block without any has mean zero.  No gradient."""
+    if torch.compiler.is_compiling():
+        return torch.ops.cutespmm.block_means(k, block, lengths)
+    return _native.op_block_means(k, block, lengths)
+
+
+def block_scores(q: torch.Tensor, means: torch.Tensor) -> torch.Tensor:
+    """Scores [batch, kv_heads, queries, blocks] (float32) of queries [batch, queries, heads, dim] against mean keys: the dot products of
+    the query heads that share a head of keys, added up.  No gradient: a selection has none."""
+    if torch.compiler.is_compiling():
+        return torch.ops.cutespmm.block_scores(q, means)
+    return _native.op_block_scores(q, means)
+
+
+def select_blocks(scores: torch.Tensor, count: int, block: int, keys: int, visible: torch.Tensor | None = None, first: int = 1, last: int = 1) -> torch.Tensor:
+    """The blocks each query attends to: int32 [batch, kv_heads, queries, count], ascending, -1 behind the last.  Chosen are the `first` first
+    and the `last` last of the blocks that the query sees, then those it sees of the highest scores (of equal ones the lowest index; a
+    block whose score is NaN or -infinity only if it is one of the first or last).
+
+    visible: int32 [batch, queries], how many keys each query sees (the first that many; 0 for a padded position); None: causal, the last
+    query sees all `keys` of them, each before it one less."""
+    if torch.compiler.is_compiling():
+        return torch.ops.cutespmm.select_blocks(scores, count, block, keys, visible, first, last)
+    return _native.op_select_blocks(scores, count, block, keys, visible, first, last)
+
+
+def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, block: int, visible: torch.Tensor | None = None,
+                    scale: float | None = None, pages: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over the visible keys of each query's blocks: softmax(scale * q k^T) v, [batch, queries, heads, dim], zero for a query that
+    sees none.  scale is positive and defaults to 1 / sqrt(dim).
+
+    q: [batch, queries, heads, dim]; k, v: [batch, keys, kv_heads, dim]; float16 or bfloat16, dim a multiple of 8 up to 128, heads a
+    multiple of kv_heads (up to 128 times).  blocks: int32 [batch, kv_heads, queries, count], count at most 128, a set of blocks of `block` keys (16, 32, 64,
+    128) for each query, as `select_blocks` returns it: any order, an index outside the keys names nothing, a repeated one counts once.
+    visible: as in `select_blocks`.  Keys that a query does not see have no effect on it, whatever their values.
+
+    A paged cache: pages int32 [batch, pages of a sequence], k and v [number of pages, block, kv_heads, dim]; block j of sequence b is
+    page pages[b, j] (an entry that is no page holds no keys), and visible says how many keys are written.  No gradient then.
+
+    Differentiable with respect to q, k and v.  The gradients' sums have a fixed order: the same bits in every run."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(q.shape[-1], 1))
+    if torch.compiler.is_compiling():
+        return torch.ops.cutespmm.block_attention(q, k, v, blocks, block, visible, scale, pages)[0]
+    return _native.op_block_attention(q, k, v, blocks, block, visible, scale, pages)
+
+
+def pattern_status() -> int:
+    """Status word of the kernels behind these functions on the current device: 0, or not if a bounded wait gave up since the last call
+    (results since then are not to be trusted).  Waits for the device."""
+    return _native.pattern_status()
+
+
+@torch.library.register_fake("cutespmm::embedding")
+def _(tokens: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
+    return table.new_empty((*tokens.shape, table.shape[1]))
+
+
+@torch.library.register_fake("cutespmm::embedding_grad")
+def _(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
+    return dout.new_empty((vocab, dout.shape[-1]))
+
+
+@torch.library.register_fake("cutespmm::block_means")
+def _(k: torch.Tensor, block: int, lengths: torch.Tensor | None) -> torch.Tensor:
+    return k.new_empty((k.shape[0], (k.shape[1] + block - 1) // block, k.shape[2], k.shape[3]))
+
+
+@torch.library.register_fake("cutespmm::block_scores")
+def _(q: torch.Tensor, means: torch.Tensor) -> torch.Tensor:
+    return q.new_empty((q.shape[0], means.shape[2], q.shape[1], means.shape[1]), dtype=torch.float32)
+
+
+@torch.library.register_fake("cutespmm::select_blocks")
+def _(scores: torch.Tensor, count: int, block: int, keys: int, visible: torch.Tensor | None, first: int, last: int) -> torch.Tensor:
+    return scores.new_empty((*scores.shape[:3], count), dtype=torch.int32)
+
+
+@torch.library.register_fake("cutespmm::block_attention")
+def _(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, block: int, visible: torch.Tensor | None, scale: float, pages: torch.Tensor | None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+@torch.library.register_fake("cutespmm::block_attention_grad")
+def _(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, blocks: torch.Tensor, block: int, visible: torch.Tensor | None, scale: float):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)

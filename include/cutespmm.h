@@ -259,6 +259,82 @@ int cutespmm_spmm_csr_noalloc(uint32_t M, uint32_t K, uint32_t nnz, const uint32
                               const uint32_t *cols_dev, const float *vals_dev, const float *B_dev, uint64_t ldb,
                               float *C_dev, uint64_t ldc, uint32_t N, void *stream);
 
+/* ---- operators whose sparse pattern the data choose in each call --------------------------------
+ * No counterpart in the reference.  A plan serves a matrix that stays; the operators below multiply with matrices that are
+ * different in every call and given by indices: the one-hot matrix of a sequence of tokens (embedding and its gradient), and the
+ * pattern "which blocks of keys does this query look at" (attention over selected blocks).  They keep nothing between calls: no
+ * plan, no state, no allocation (where a call needs scratch, the caller passes it).  Device pointers refer to the current CUDA
+ * device, work is ordered on `stream`, nothing waits for the device; calls may overlap on any streams and be captured.
+ *
+ * Elements are fp32, fp16 or bf16; sums are held in fp32 and rounded once. */
+typedef enum { CUTESPMM_F32 = 0, CUTESPMM_F16 = 1, CUTESPMM_BF16 = 2 } cutespmm_dtype_t;
+
+/* out[i] = scale * table[tokens[i]] for i < count: rows of dim elements, leading dimensions in elements.  tokens: int32 or int64
+ * (token_bytes 4 or 8).  A token outside [0, vocab) -- a padded position, say -- names no row: its row of out is zero. */
+int cutespmm_embedding(int dtype, const void *table_dev, uint64_t ld_table, uint64_t vocab, uint32_t dim, const void *tokens_dev,
+                       int token_bytes, uint64_t count, float scale, void *out_dev, uint64_t ld_out, void *stream);
+/* dtable[v] = scale * sum of dout[i] over the i with tokens[i] = v: every row of dtable (vocab x dim) is written, zeros where no
+ * token names it.  The tokens are sorted on the device in the call and a row's terms added in the order of their positions (long
+ * sums as partial sums of fixed ranges of the sorted positions): the same bits in every run.  count, vocab < 2^31.  workspace:
+ * cutespmm_embedding_grad_workspace() bytes, 256-byte aligned, not shared with a call that may overlap. */
+uint64_t cutespmm_embedding_grad_workspace(uint64_t count, uint64_t vocab, uint32_t dim);
+int cutespmm_embedding_grad(int dtype, const void *dout_dev, uint64_t ld_dout, const void *tokens_dev, int token_bytes, uint64_t count,
+                            uint64_t vocab, uint32_t dim, float scale, void *dtable_dev, uint64_t ld_dtable, void *workspace_dev,
+                            uint64_t workspace_bytes, void *stream);
+
+/* Attention over selected blocks.  Keys are cut into blocks of `block` (16, 32, 64 or 128) consecutive ones; kv_heads heads of keys
+ * and values serve `heads` = group * kv_heads query heads, head h using head h / group of the keys.  dim: a multiple of 8, at most
+ * 128.  q, k, v and the means are fp16 or bf16.  Operands are [batch][row][head][dim] with strides in elements, dim contiguous,
+ * strides multiples of 8 and pointers 16-byte aligned.
+ *
+ * visible[b][t]: how many keys query t of sequence b sees -- the first that many; 0: the query is padding and its output zero;
+ * clamped to [0, keys].  NULL: causal, the last query sees every key (query t sees keys - queries + 1 + t). */
+typedef struct {
+    uint32_t struct_size;  /* sizeof(cutespmm_block_attention_t) */
+    uint32_t dtype;        /* CUTESPMM_F16 or CUTESPMM_BF16 */
+    uint32_t batch, queries, heads, kv_heads, dim, keys;
+    uint32_t block;        /* keys per block */
+    uint32_t count;        /* blocks per query, at most 128 */
+    const void *q, *k, *v;
+    int64_t q_strides[3], k_strides[3], v_strides[3];  /* batch (a paged cache: page), row, head */
+    const int32_t *blocks;   /* batch x kv_heads x queries x count, contiguous: the set of blocks of each query.  Any order; an
+                                index outside [0, ceil(keys / block)) names nothing, one that stands there twice counts once */
+    const int32_t *visible;  /* batch x queries, contiguous, or NULL */
+    /* paged cache: k and v are [num_pages][block][kv_heads][dim] and block j of sequence b is page pages[b][j]; keys = page_cols *
+     * block.  An entry outside [0, num_pages) holds no keys.  NULL and zeros otherwise. */
+    const int32_t *pages;    /* batch x page_cols, contiguous */
+    uint32_t page_cols, num_pages;
+    float scale;             /* of the scores, positive; usually 1 / sqrt(dim) */
+} cutespmm_block_attention_t;
+
+/* means[b][j][h] = mean of the keys of block j (of the first lengths[b] keys where lengths is not NULL; 0 for a block without any),
+ * in the keys' type; batch x ceil(keys / block) x kv_heads x dim, contiguous. */
+int cutespmm_block_means(int dtype, const void *k_dev, const int64_t k_strides[3], const int32_t *lengths_dev, uint32_t batch, uint32_t keys,
+                         uint32_t kv_heads, uint32_t dim, uint32_t block, void *means_dev, void *stream);
+/* scores[b][h][t][j] = sum over the query heads of group h of <q[b][t][head], means[b][j][h]>, fp32, contiguous. */
+int cutespmm_block_scores(int dtype, const void *q_dev, const int64_t q_strides[3], const void *means_dev, const int64_t means_strides[3],
+                          uint32_t batch, uint32_t queries, uint32_t heads, uint32_t kv_heads, uint32_t blocks, uint32_t dim, float *scores_dev,
+                          void *stream);
+/* blocks[b][h][t]: `count` indices in ascending order, -1 behind the last -- the first `first` and the last `last` of the blocks the
+ * query sees, then those it sees of the highest scores (equal scores: the lowest index; NaN and -infinity are never chosen).
+ * first + last <= count; at most 16384 blocks.  s_strides: elements of scores per batch, head, query; a row is contiguous. */
+int cutespmm_select_blocks(const float *scores_dev, const int64_t s_strides[3], const int32_t *visible_dev, uint32_t batch, uint32_t kv_heads,
+                           uint32_t queries, uint32_t blocks, uint32_t keys, uint32_t block, uint32_t count, uint32_t first, uint32_t last,
+                           int32_t *blocks_dev, void *stream);
+/* out[b][t][h] = softmax(scale * <q, k>) v over the visible keys of the query's blocks (zero where there are none), batch x queries x
+ * heads x dim, contiguous; lse[b][h][t]: the logarithm of the sum of exponentials (-infinity where there are none). */
+int cutespmm_block_attention(const cutespmm_block_attention_t *args, void *out_dev, float *lse_dev, void *stream);
+/* Gradients with respect to q, k and v (contiguous, shaped like them) from out, lse and dout (dout_strides as q's).  Not for a paged
+ * cache.  Sums have a fixed order.  workspace: cutespmm_block_attention_grad_workspace() bytes, 256-byte aligned, not shared with a
+ * call that may overlap. */
+uint64_t cutespmm_block_attention_grad_workspace(const cutespmm_block_attention_t *args);
+int cutespmm_block_attention_grad(const cutespmm_block_attention_t *args, const void *dout_dev, const int64_t dout_strides[3],
+                                  const void *out_dev, const float *lse_dev, void *dq_dev, void *dk_dev, void *dv_dev, void *workspace_dev,
+                                  uint64_t workspace_bytes, void *stream);
+/* Status word that these operators' kernels write on the current device when a bounded wait gives up (0 = none), cleared by the
+ * read.  Waits for the device. */
+int cutespmm_pattern_status(uint32_t *status);
+
 /* Number of kernels one cutespmm_spmm call launches for this plan and N, the padding of B included, on contiguous operands
  * (ldb = ldc = N) that start on a 16-byte boundary, outside a capture and with memory for the padded copy. */
 int cutespmm_spmm_launch_count(const cutespmm_plan_t *plan, uint32_t N);
