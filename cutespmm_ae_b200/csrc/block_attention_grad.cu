@@ -260,8 +260,9 @@ struct GradLayout {
         const uint64_t pairs = (uint64_t)a.batch * a.kv_heads * a.queries * a.count * (a.block > kKeyTile ? 2 : 1);
         uint64_t rows = pairs * group / 4096;  // about 4096 items in large jobs
         if (rows < kItemRows) rows = kItemRows;
-        item_queries = (uint32_t)(rows / group < a.queries ? rows / group : a.queries);
-        if (item_queries == 0) item_queries = 1;
+        const uint32_t per_tile = 128 / group;  // queries of 128 rows
+        uint64_t n = rows / group < a.queries ? rows / group : a.queries;
+        item_queries = (uint32_t)((n + per_tile - 1) / per_tile * per_tile);
         max_items = pairs / item_queries + tile_rows;
         max_slots = 2 * (pairs / item_queries) + 1;  // a tile with two items or more has more than half of them full
         uint64_t at = 0;
@@ -330,6 +331,18 @@ __global__ void __launch_bounds__(256) pattern_count_kernel(TurnArgs p)
     if ((threadIdx.x & 31) == 0) p.counts[row] = n;
 }
 
+// Work item it: its first query, as a rank among those that name the tile, and how many it takes -- equal parts, whole tiles of rows.
+__device__ __forceinline__ uint2 item_part(const TurnArgs &p, uint2 it)
+{
+    const uint32_t n = p.counts[it.x], parts = (n + p.item_queries - 1) / p.item_queries, per_tile = 128 / (p.a.heads / p.a.kv_heads);
+    const uint32_t each = ((n + parts - 1) / parts + per_tile - 1) / per_tile * per_tile, first = it.y * each;
+    return make_uint2(first, min(each, n - first));
+}
+__device__ __forceinline__ void copy16(uint32_t saddr, uint64_t src, uint32_t bytes)  // what is behind `bytes` becomes zeros
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(src), "r"(bytes) : "memory");
+}
+
 // One block: the work items of every tile, in order; slots for partial sums where a tile has several.
 __global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
 {
@@ -372,16 +385,16 @@ __global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
 }
 
 // ---- dk and dv ---------------------------------------------------------------------------------------------------------
-// One thread block per SM walks work items: 64 keys and a range of the queries that name them.  The queries' rows of q and dout (all heads of
-// the group: a TMA box each) are gathered into tiles of 128 rows; per tile
+// One thread block per SM walks work items: 64 keys and a range of the queries that name them.  The queries' rows of q and dout are
+// gathered into tiles of 128 rows (16 bytes a lane; a TMA box per query and 64 dims took 9100 cycles a tile, a hundred each to issue); per tile
 //     S  = Q K^T   and  D = dO V^T       (128 x 64 each, tensor memory, two buffers)
 //     P, dS in registers of eight warps (thread = row: lse, delta and the limit of the row are one value each), written as 16-bit operands
 //     dV^T += dO^T P  and  dK^T += Q^T dS  (dims x 64 keys, accumulators in tensor memory for the whole item)
 // with the same shared-memory bytes of Q and dO serving as row-major operand of the first pair and as transposed operand of the second.
 // The tile after is multiplied while this one's P and dS are formed.  Every query names its keys by choice, so no row of a tile is
 // wasted, however little neighbouring queries agree; this is what makes the 128-row instruction the right one here.
-constexpr int kDkvWarps = 8;  // softmax warps; warp 8 loads, warp 9 multiplies
-constexpr int kDkvThreads = (kDkvWarps + 2) * 32;
+constexpr int kDkvWarps = 8, kDkvLoaders = 4;  // warps 0-7 form P and dS, 8-11 load, warp 12 multiplies
+constexpr int kDkvThreads = (kDkvWarps + kDkvLoaders + 1) * 32;
 constexpr int kDkvStages = 2;
 constexpr uint32_t kTmemS = 0, kTmemD = 64, kTmemBuffer = 128, kTmemDv = 256, kTmemDk = 320, kTmemCols = 512;
 
@@ -393,20 +406,20 @@ template <int DP> struct DkvSmem {
     static constexpr int kStage = kValues + kHalves * 64 * 128;         // per stage q, then dout
     static constexpr int kP = kStage + kDkvStages * 2 * kTileBytes;     // 128 rows x 64 keys
     static constexpr int kDs = kP + 128 * 128;
-    static constexpr int kLists = kDs + 128 * 128;                      // per stage the queries of a tile
-    static constexpr int kBars = kLists + kDkvStages * 128 * 4;
+    static constexpr int kRows = kDs + 128 * 128;                       // per stage and row: lse log2 e, delta, a bit per key that it looks at
+    static constexpr int kBars = kRows + kDkvStages * 128 * 16;
     static constexpr int kBytes = kBars + 16 * 8 + 16;
 };
 
 template <class T, int DP>
 __global__ void __launch_bounds__(kDkvThreads, 1)
-    block_attention_dkv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap do_map, TurnArgs p)
+    block_attention_dkv_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, TurnArgs p)
 {
     using S = DkvSmem<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const AttentionArgs &a = p.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars);  // q and dout of a stage have landed, its list is written
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars);  // q, dout and the rows of a stage are there
     uint64_t *empty = full + kDkvStages;                             // the products that read the stage are done
     uint64_t *kv_full = empty + kDkvStages;
     uint64_t *scored = kv_full + 1;                                  // S and D of a buffer are complete (2)
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + S::kBars + 16 * 8);  // [0] tensor memory, [1] gave up
     if (threadIdx.x == 0) {
         for (int s = 0; s < kDkvStages; ++s) {
-            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&full[s], kDkvLoaders);
             ptx::mbar_init(&empty[s], 1);
         }
         ptx::mbar_init(kv_full, 1);
@@ -430,10 +443,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         misc[1] = 0;
         ptx::fence_mbar_init();
     }
-    // rows of a tile behind its last query are never loaded: zeros for good
-    for (int i = threadIdx.x; i < kDkvStages * 2 * S::kTileBytes / 16; i += kDkvThreads) reinterpret_cast<uint4 *>(smem + S::kStage)[i] = make_uint4(0, 0, 0, 0);
     if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kTmemCols);
-    ptx::fence_async_smem();
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -445,95 +455,134 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     const uint32_t items = p.totals[0];
     uint32_t tile_count = 0;  // tiles of all items so far
     bool ok = true;
-    auto tiles_of = [&](uint2 it) {
-        const uint32_t n = min(p.counts[it.x] - it.y * p.item_queries, p.item_queries);
-        return (n + per_tile - 1) / per_tile;
-    };
+    auto tiles_of = [&](uint2 it) { return (item_part(p, it).y + per_tile - 1) / per_tile; };
 
-    if (warp == kDkvWarps) {
-        // ================= loads =================
+    if (warp >= kDkvWarps && warp < kDkvWarps + kDkvLoaders) {
+        // ================= loads: warp w brings rows 32 w .. 32 w + 31 of every tile =================
+        const uint32_t w = warp - kDkvWarps, r = w * 32 + lane, entry = r / group, head = r % group;
+        const uint32_t blocks_per_tile = a.block < kKeyTile ? kKeyTile / a.block : 1;
+        uint32_t issued = 0, announced = 0;  // tiles whose copies are queued, and those the others know of
+        // Announces the tile whose copies are in flight, if there is one.  Always before this warp waits for anything: what it waits for
+        // comes from products that are queued behind those of that tile.
+        auto announce = [&]() {
+            if (issued == announced) return;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            ptx::fence_async_smem();  // the tensor cores read what this thread's copies wrote
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&full[announced % kDkvStages]);
+            ++announced;
+        };
         for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
             const uint2 it = p.items[i];
             const uint32_t tile = it.x % p.tiles, bh = it.x / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
-            const uint32_t n_tiles = tiles_of(it);
-            uint32_t left = min(p.counts[it.x] - it.y * p.item_queries, p.item_queries);
-            if (k && !(ok = ptx::mbar_wait(summed, (k - 1) & 1u))) break;
-            if (lane == 0) {
-                ptx::mbar_expect_tx(kv_full, 2 * S::kHalves * 64 * 128);
-                for (int h = 0; h < S::kHalves; ++h) {
-                    tc::tma_load4(smem + S::kKeys + h * 64 * 128, &k_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
-                    tc::tma_load4(smem + S::kValues + h * 64 * 128, &v_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
+            const uint2 part = item_part(p, it);  // ranks among the queries that name the tile
+            const uint32_t n_tiles = (part.y + per_tile - 1) / per_tile;
+            announce();
+            if (w == 0) {
+                if (k && !(ok = ptx::mbar_wait(summed, (k - 1) & 1u))) break;
+                if (lane == 0) {
+                    ptx::mbar_expect_tx(kv_full, 2 * S::kHalves * 64 * 128);
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        tc::tma_load4(smem + S::kKeys + h * 64 * 128, &k_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
+                        tc::tma_load4(smem + S::kValues + h * 64 * 128, &v_map, h * 64, (int)kv, (int)(tile * kKeyTile), (int)b, kv_full);
+                    }
                 }
+                __syncwarp();
             }
-            // a window of 32 words of the tile's bits, one per lane; the queries of earlier items are passed over
-            uint32_t skip = it.y * p.item_queries, window = 0, word = 0;
-            auto next_window = [&]() {
+            // a window of 32 words of the tile's bits, one per lane: `before` queries in front of this lane's word, `ranks` in front of the window
+            uint32_t window = 0, word = 0, before = 0, size = 0, ranks = 0;
+            auto take_window = [&]() {
                 word = window + lane < p.words ? tile_word(p, it.x, window + lane) : 0u;
-                window += 32;
+                before = __popc(word);
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(~0u, before, d);
+                    if (lane >= (uint32_t)d) before += up;
+                }
+                size = __shfl_sync(~0u, before, 31);
+                before -= __popc(word);
             };
-            next_window();
-            for (;;) {
-                const uint32_t n = __reduce_add_sync(~0u, __popc(word));
-                if (n > skip || window >= p.words) break;
-                skip -= n;
-                next_window();
-            }
+            take_window();
+            const T *q0 = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(kv * group + head) * a.q_head;
+            const T *g0 = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(kv * group + head) * a.do_head;
+            const uint64_t stat0 = ((uint64_t)b * a.heads + kv * group + head) * a.queries;
             for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
+                // this lane's row: the query of rank part.x + j per_tile + entry
+                const uint32_t local = j * per_tile + entry, rank = part.x + local;
+                uint32_t t = a.queries;
+                bool pending = entry < per_tile && local < part.y;
+                for (;;) {
+                    const bool here = pending && rank < ranks + size;
+                    if (__any_sync(~0u, here)) {
+                        const uint32_t at = here ? rank - ranks : 0u;
+                        uint32_t l = 0;
+#pragma unroll
+                        for (int d = 16; d; d >>= 1)
+                            if (__shfl_sync(~0u, before, l + d) <= at) l += d;
+                        uint32_t bits = __shfl_sync(~0u, word, l), nth = at - __shfl_sync(~0u, before, l), bit = 0;
+#pragma unroll
+                        for (int d = 16; d; d >>= 1) {
+                            const uint32_t c = __popc(bits & ((1u << d) - 1u));
+                            if (nth >= c) {
+                                nth -= c;
+                                bits >>= d;
+                                bit += d;
+                            }
+                        }
+                        if (here) {
+                            t = (window + l) * 32 + bit;
+                            pending = false;
+                        }
+                    }
+                    if (!__any_sync(~0u, pending) || window + 32 >= p.words) break;
+                    ranks += size;
+                    window += 32;
+                    take_window();
+                }
+                const bool on = t < a.queries;
+                float lse = 0.f, delta = 0.f;
+                uint64_t sees = 0;
+                if (on) {
+                    lse = a.lse[stat0 + t] * kLog2e;
+                    delta = a.delta[stat0 + t];
+                    const int limit = (int)visible_keys(a, b, t) - (int)(tile * kKeyTile);
+                    sees = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1ull : 0ull;
+                    if (blocks_per_tile > 1) {
+                        uint64_t named = 0;
+                        const uint64_t one = (1ull << a.block) - 1ull;
+                        for (uint32_t n = 0; n < blocks_per_tile && tile * blocks_per_tile + n < a.num_blocks; ++n)
+                            if ((p.bits[((uint64_t)bh * a.num_blocks + tile * blocks_per_tile + n) * p.words + (t >> 5)] >> (t & 31)) & 1u) named |= one << (n * a.block);
+                        sees &= named;
+                    }
+                }
+                announce();  // the tile before has had all of this one's look-up to land
                 const uint32_t s = tile_count % kDkvStages;
                 if (!(ok = ptx::mbar_wait(&empty[s], ((tile_count / kDkvStages) & 1u) ^ 1u))) break;
-                uint32_t *list = reinterpret_cast<uint32_t *>(smem + S::kLists) + s * 128;
-                const uint32_t want = min(per_tile, left);
-                uint32_t got = 0;
-                while (got < want) {
-                    const uint32_t mine = __popc(word);
-                    uint32_t at = mine;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const uint32_t up = __shfl_up_sync(~0u, at, d);
-                        if (lane >= (uint32_t)d) at += up;
-                    }
-                    const uint32_t n = __shfl_sync(~0u, at, 31);
-                    at -= mine;
-                    // this lane's queries have ranks at, at + 1, ... in the window; ranks below `skip` are passed over
-                    const uint32_t end = min(n, skip + want - got);
-                    for (; word && at < end; ++at) {
-                        const uint32_t bit = __ffs(word) - 1;
-                        word &= word - 1;
-                        if (at >= skip) list[got + at - skip] = (window - 32 + lane) * 32 + bit;
-                    }
-                    got += end > skip ? end - skip : 0u;
-                    skip = 0;
-                    if (got < want) {
-                        if (window >= p.words) break;  // cannot be: the counts are those of these bits
-                        next_window();
-                    }
+                reinterpret_cast<uint4 *>(smem + S::kRows)[s * 128 + r] = make_uint4(__float_as_uint(lse), __float_as_uint(delta), (uint32_t)sees, (uint32_t)(sees >> 32));
+                const uint64_t q_at = reinterpret_cast<uint64_t>(q0 + (int64_t)(on ? t : 0u) * a.q_query), g_at = reinterpret_cast<uint64_t>(g0 + (int64_t)(on ? t : 0u) * a.do_query);
+                const uint32_t q = ptx::smem_u32(smem + S::kStage) + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
+                constexpr uint32_t kPieces = DP / 8, kAtOnce = 32 / kPieces;  // 16-byte pieces of a row, rows of an instruction
+                const uint32_t piece = lane % kPieces;
+#pragma unroll 8
+                for (uint32_t x = 0; x < 32; x += kAtOnce) {
+                    const uint32_t from = x + lane / kPieces, row = w * 32 + from;
+                    const uint64_t qs = __shfl_sync(~0u, q_at, from), gs = __shfl_sync(~0u, g_at, from);
+                    const uint32_t bytes = __shfl_sync(~0u, (uint32_t)on, from) && piece * 8 < a.dim ? 16u : 0u;  // 0: zeros
+                    const uint32_t at = (piece >> 3) * 128 * 128 + tc::swizzled(row, piece & 7);
+                    copy16(q + at, bytes ? qs + piece * 16 : reinterpret_cast<uint64_t>(a.q), bytes);
+                    copy16(g + at, bytes ? gs + piece * 16 : reinterpret_cast<uint64_t>(a.dout), bytes);
                 }
-                for (uint32_t r = got + lane; r < per_tile; r += 32) list[r] = a.queries;  // no such query: its rows arrive as zeros
-                left -= want;
-                __syncwarp();
-                if (lane == 0) ptx::mbar_expect_tx(&full[s], per_tile * group * 128 * S::kHalves * 2);
-                __syncwarp();
-                unsigned char *q = smem + S::kStage + s * 2 * S::kTileBytes, *g = q + S::kTileBytes;
-                for (uint32_t r = lane; r < per_tile; r += 32) {
-                    const int t = (int)list[r];
-#pragma unroll
-                    for (int h = 0; h < S::kHalves; ++h) {
-                        const uint32_t at = h * 128 * 128 + r * group * 128;
-                        tc::tma_load4(q + at, &q_map, h * 64, (int)(kv * group), t, (int)b, &full[s]);
-                        tc::tma_load4(g + at, &do_map, h * 64, (int)(kv * group), t, (int)b, &full[s]);
-                    }
-                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ++issued;
             }
         }
+        announce();
         if (!ok) {
             misc[1] = 1;
-            if (lane == 0) {  // no copy stays in flight
-                ptx::mbar_wait(kv_full, 0);
-                ptx::mbar_wait(kv_full, 1);
-                for (uint32_t j = tile_count > kDkvStages ? tile_count - kDkvStages : 0; j < tile_count; ++j) ptx::mbar_wait(&full[j % kDkvStages], (j / kDkvStages) & 1u);
-            }
+            if (w == 0 && lane == 0)  // no copy stays in flight
+                for (uint32_t x = 0; x < 2; ++x) ptx::mbar_wait(kv_full, x);
         }
-    } else if (warp == kDkvWarps + 1) {
+    } else if (warp == kDkvWarps + kDkvLoaders) {
         // ================= products =================
         if (lane == 0) {
             constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -580,36 +629,19 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         }
     } else {
         // ================= P and dS =================
-        const uint32_t r = (warp & 3) * 32 + lane, half = warp >> 2, entry = r / group, head = r % group;
+        const uint32_t r = (warp & 3) * 32 + lane, half = warp >> 2;
         const float scale_log2 = a.scale * kLog2e;
         const uint32_t lanes = tmem + (((warp & 3) * 32) << 16);
         for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
             const uint2 it = p.items[i];
             const uint32_t tile = it.x % p.tiles, bh = it.x / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
             const uint32_t n_tiles = tiles_of(it);
-            const uint32_t blocks_per_tile = a.block < kKeyTile ? kKeyTile / a.block : 1, block0 = tile * kKeyTile / a.block;
             for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
                 const uint32_t s = tile_count % kDkvStages;
                 if (!(ok = ptx::mbar_wait(&full[s], (tile_count / kDkvStages) & 1u))) break;
-                const uint32_t t = entry < per_tile ? reinterpret_cast<const uint32_t *>(smem + S::kLists)[s * 128 + entry] : a.queries;
-                const bool on = t < a.queries;
-                float lse = 0.f, delta = 0.f;
-                int limit = 0;
-                uint32_t named = 0;  // which blocks of the tile the query names
-                if (on) {
-                    const uint64_t at = ((uint64_t)b * a.heads + kv * group + head) * a.queries + t;
-                    lse = a.lse[at] * kLog2e;
-                    delta = a.delta[at];
-                    limit = (int)visible_keys(a, b, t) - (int)(tile * kKeyTile) - (int)half * 32;
-                    if (blocks_per_tile == 1) named = 1;
-                    else
-                        for (uint32_t n = 0; n < blocks_per_tile && block0 + n < a.num_blocks; ++n)
-                            named |= ((p.bits[((uint64_t)bh * a.num_blocks + block0 + n) * p.words + (t >> 5)] >> (t & 31)) & 1u) << n;
-                }
-                // a bit per key of this thread's half
-                uint32_t sees = limit >= 32 ? ~0u : limit > 0 ? (1u << limit) - 1u : 0u;
-                if (blocks_per_tile == 2) sees = (named >> half) & 1u ? sees : 0u;
-                if (blocks_per_tile == 4) sees &= ((named >> (2 * half)) & 1u ? 0xffffu : 0u) | ((named >> (2 * half + 1)) & 1u ? 0xffff0000u : 0u);
+                const uint4 info = reinterpret_cast<const uint4 *>(smem + S::kRows)[s * 128 + r];
+                const float lse = __uint_as_float(info.x), delta = __uint_as_float(info.y);
+                const uint32_t sees = half ? info.w : info.z;  // a bit per key of this thread's half
                 const uint32_t buffer = lanes + (tile_count & 1u) * kTmemBuffer + half * 32;
                 if (!(ok = ptx::mbar_wait(&scored[tile_count & 1u], (tile_count >> 1) & 1u))) break;
                 tc::fence_after();
@@ -754,15 +786,12 @@ template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count
     if ((e = launch_overlapped(pattern_bits_kernel, dim3((unsigned)((bit_warps + 7) / 8)), dim3(256), 0, s, p)) != cudaSuccess) return e;
     if ((e = launch_overlapped(pattern_count_kernel, dim3((unsigned)((l.tile_rows + 7) / 8)), dim3(256), 0, s, p)) != cudaSuccess) return e;
     if ((e = launch_overlapped(pattern_items_kernel, dim3(1), dim3(1024), 0, s, p)) != cudaSuccess) return e;
-    CUtensorMap k_map, v_map, q_map, do_map;
-    const uint32_t group = a.heads / a.kv_heads;
+    CUtensorMap k_map, v_map;
     if ((e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, kKeyTile)) != cudaSuccess) return e;
     if ((e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, kKeyTile)) != cudaSuccess) return e;
-    if ((e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, 1, group)) != cudaSuccess) return e;
-    if ((e = tc::make_map(&do_map, bf16, a.dout, a.dim, a.heads, a.queries, a.batch, a.do_head, a.do_query, a.do_batch, 1, group)) != cudaSuccess) return e;
     if ((e = allow_dynamic_smem<block_attention_dkv_kernel<T, DP>>(DkvSmem<DP>::kBytes)) != cudaSuccess) return e;
     const uint64_t blocks = l.max_items < (uint64_t)sm_count ? l.max_items : (uint64_t)sm_count;
-    if ((e = launch_overlapped(block_attention_dkv_kernel<T, DP>, dim3((unsigned)blocks), dim3(kDkvThreads), DkvSmem<DP>::kBytes, s, k_map, v_map, q_map, do_map, p)) != cudaSuccess) return e;
+    if ((e = launch_overlapped(block_attention_dkv_kernel<T, DP>, dim3((unsigned)blocks), dim3(kDkvThreads), DkvSmem<DP>::kBytes, s, k_map, v_map, p)) != cudaSuccess) return e;
     return launch_overlapped(dkv_join_kernel<T, DP>, dim3((unsigned)l.tile_rows), dim3(256), 0, s, p);
 }
 
