@@ -393,9 +393,10 @@ __global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
 // with the same shared-memory bytes of Q and dO serving as row-major operand of the first pair and as transposed operand of the second.
 // The tile after is multiplied while this one's P and dS are formed.  Every query names its keys by choice, so no row of a tile is
 // wasted, however little neighbouring queries agree; this is what makes the 128-row instruction the right one here.
-constexpr int kDkvWarps = 8, kDkvLoaders = 4;  // warps 0-7 form P and dS, 8-11 load, warp 12 multiplies
+constexpr int kDkvWarps = 8, kDkvLoaders = 8;  // warps 0-7 form P and dS, 8-15 load, warp 16 multiplies
 constexpr int kDkvThreads = (kDkvWarps + kDkvLoaders + 1) * 32;
 constexpr int kDkvStages = 2;
+constexpr uint32_t kPolls = 1u << 24;  // of a role that looks at two barriers in turn, before it gives up
 constexpr uint32_t kTmemS = 0, kTmemD = 64, kTmemBuffer = 128, kTmemDv = 256, kTmemDk = 320, kTmemCols = 512;
 
 template <int DP> struct DkvSmem {
@@ -458,8 +459,10 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     auto tiles_of = [&](uint2 it) { return (item_part(p, it).y + per_tile - 1) / per_tile; };
 
     if (warp >= kDkvWarps && warp < kDkvWarps + kDkvLoaders) {
-        // ================= loads: warp w brings rows 32 w .. 32 w + 31 of every tile =================
-        const uint32_t w = warp - kDkvWarps, r = w * 32 + lane, entry = r / group, head = r % group;
+        // ================= loads: warps w and w + 4 look up rows 32 w .. 32 w + 31 of every tile, one brings q, one dout =================
+        const uint32_t w = (warp - kDkvWarps) & 3, r = w * 32 + lane, entry = r / group, head = r % group;
+        const bool is_q = warp - kDkvWarps < 4;
+        const int64_t row_stride = is_q ? a.q_query : a.do_query;
         const uint32_t blocks_per_tile = a.block < kKeyTile ? kKeyTile / a.block : 1;
         uint32_t issued = 0, announced = 0;  // tiles whose copies are queued, and those the others know of
         // Announces the tile whose copies are in flight, if there is one.  Always before this warp waits for anything: what it waits for
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const uint2 part = item_part(p, it);  // ranks among the queries that name the tile
             const uint32_t n_tiles = (part.y + per_tile - 1) / per_tile;
             announce();
-            if (w == 0) {
+            if (warp == kDkvWarps) {
                 if (k && !(ok = ptx::mbar_wait(summed, (k - 1) & 1u))) break;
                 if (lane == 0) {
                     ptx::mbar_expect_tx(kv_full, 2 * S::kHalves * 64 * 128);
@@ -503,8 +506,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                 before -= __popc(word);
             };
             take_window();
-            const T *q0 = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(kv * group + head) * a.q_head;
-            const T *g0 = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(kv * group + head) * a.do_head;
+            const T *row0 = is_q ? static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(kv * group + head) * a.q_head
+                                 : static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(kv * group + head) * a.do_head;
             const uint64_t stat0 = ((uint64_t)b * a.heads + kv * group + head) * a.queries;
             for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
                 // this lane's row: the query of rank part.x + j per_tile + entry
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                 const bool on = t < a.queries;
                 float lse = 0.f, delta = 0.f;
                 uint64_t sees = 0;
-                if (on) {
+                if (on && is_q) {
                     lse = a.lse[stat0 + t] * kLog2e;
                     delta = a.delta[stat0 + t];
                     const int limit = (int)visible_keys(a, b, t) - (int)(tile * kKeyTile);
@@ -558,19 +561,18 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                 announce();  // the tile before has had all of this one's look-up to land
                 const uint32_t s = tile_count % kDkvStages;
                 if (!(ok = ptx::mbar_wait(&empty[s], ((tile_count / kDkvStages) & 1u) ^ 1u))) break;
-                reinterpret_cast<uint4 *>(smem + S::kRows)[s * 128 + r] = make_uint4(__float_as_uint(lse), __float_as_uint(delta), (uint32_t)sees, (uint32_t)(sees >> 32));
-                const uint64_t q_at = reinterpret_cast<uint64_t>(q0 + (int64_t)(on ? t : 0u) * a.q_query), g_at = reinterpret_cast<uint64_t>(g0 + (int64_t)(on ? t : 0u) * a.do_query);
-                const uint32_t q = ptx::smem_u32(smem + S::kStage) + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
+                if (is_q) reinterpret_cast<uint4 *>(smem + S::kRows)[s * 128 + r] = make_uint4(__float_as_uint(lse), __float_as_uint(delta), (uint32_t)sees, (uint32_t)(sees >> 32));
+                const uint64_t row_at = reinterpret_cast<uint64_t>(row0 + (int64_t)(on ? t : 0u) * row_stride);
+                const uint32_t to = ptx::smem_u32(smem + S::kStage) + (2 * s + (is_q ? 0 : 1)) * S::kTileBytes;
                 constexpr uint32_t kPieces = DP / 8, kAtOnce = 32 / kPieces;  // 16-byte pieces of a row, rows of an instruction
                 const uint32_t piece = lane % kPieces;
-#pragma unroll 8
+                const uint32_t rows_on = __ballot_sync(~0u, on);
+#pragma unroll
                 for (uint32_t x = 0; x < 32; x += kAtOnce) {
-                    const uint32_t from = x + lane / kPieces, row = w * 32 + from;
-                    const uint64_t qs = __shfl_sync(~0u, q_at, from), gs = __shfl_sync(~0u, g_at, from);
-                    const uint32_t bytes = __shfl_sync(~0u, (uint32_t)on, from) && piece * 8 < a.dim ? 16u : 0u;  // 0: zeros
-                    const uint32_t at = (piece >> 3) * 128 * 128 + tc::swizzled(row, piece & 7);
-                    copy16(q + at, bytes ? qs + piece * 16 : reinterpret_cast<uint64_t>(a.q), bytes);
-                    copy16(g + at, bytes ? gs + piece * 16 : reinterpret_cast<uint64_t>(a.dout), bytes);
+                    const uint32_t from = x + lane / kPieces;
+                    const uint64_t src = __shfl_sync(~0u, row_at, from);
+                    const uint32_t bytes = ((rows_on >> from) & 1u) && piece * 8 < a.dim ? 16u : 0u;  // 0: zeros
+                    copy16(to + (piece >> 3) * 128 * 128 + tc::swizzled(w * 32 + from, piece & 7), bytes ? src + piece * 16 : reinterpret_cast<uint64_t>(a.q), bytes);
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 ++issued;
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         announce();
         if (!ok) {
             misc[1] = 1;
-            if (w == 0 && lane == 0)  // no copy stays in flight
+            if (warp == kDkvWarps && lane == 0)  // no copy stays in flight
                 for (uint32_t x = 0; x < 2; ++x) ptx::mbar_wait(kv_full, x);
         }
     } else if (warp == kDkvWarps + kDkvLoaders) {
@@ -590,40 +592,43 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const uint32_t base = ptx::smem_u32(smem);
             // dims as rows: with 64 of them the second block of the 128-row instruction is the first once more, and its rows are left alone
             constexpr uint32_t block_bytes = DP == 128 ? 128 * 128 : 0;
-            uint32_t done = 0;  // tiles whose second products are issued
-            auto second = [&](uint32_t k, bool first, bool last) {
-                const uint32_t s = done % kDkvStages;
-                ok = ptx::mbar_wait(formed, done & 1u) && (!first || !k || ptx::mbar_wait(read, (k - 1) & 1u));
-                if (!ok) return;
-                tc::fence_after();
-                const uint32_t q = base + S::kStage + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
-#pragma unroll
-                for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDv, tc::desc_mn(g + r * 2048, block_bytes), tc::desc_mn(base + S::kP + r * 2048, 0), id_t, !first || r);
-#pragma unroll
-                for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDk, tc::desc_mn(q + r * 2048, block_bytes), tc::desc_mn(base + S::kDs + r * 2048, 0), id_t, !first || r);
-                tc::commit(&empty[s]);
-                tc::commit(used);
-                if (last) tc::commit(summed);
-                ++done;
-            };
+            // every descriptor is one of these plus a constant
+            const uint64_t q_k = tc::desc_k(base + S::kStage), k_k = tc::desc_k(base + S::kKeys), v_k = tc::desc_k(base + S::kValues);
+            const uint64_t q_mn = tc::desc_mn(base + S::kStage, block_bytes), p_mn = tc::desc_mn(base + S::kP, 0), d_mn = tc::desc_mn(base + S::kDs, 0);
+            constexpr uint32_t kTile = S::kTileBytes >> 4;
+            uint32_t scores = 0, sums = 0;  // tiles whose first and second products are issued, over all items
             for (uint32_t k = 0, i = blockIdx.x; i < items && ok; i += gridDim.x, ++k) {
-                const uint32_t n_tiles = tiles_of(p.items[i]);
+                const uint32_t first = scores, end = first + tiles_of(p.items[i]);
                 if (!(ok = ptx::mbar_wait(kv_full, k & 1u))) break;
-                for (uint32_t j = 0; j < n_tiles && ok; ++j, ++tile_count) {
-                    const uint32_t s = tile_count % kDkvStages, buffer = tmem + (tile_count & 1u) * kTmemBuffer;
-                    if (!(ok = ptx::mbar_wait(&full[s], (tile_count / kDkvStages) & 1u))) break;
-                    tc::fence_after();
-                    const uint32_t q = base + S::kStage + s * 2 * S::kTileBytes, g = q + S::kTileBytes;
+                // whichever is ready: the second products of a tile give its stage back, so they go first
+                for (uint32_t idle = 0; sums < end;) {
+                    if (sums < scores && ptx::mbar_test(formed, sums & 1u)) {
+                        if (sums == first && k && !(ok = ptx::mbar_wait(read, (k - 1) & 1u))) break;
+                        tc::fence_after();
+                        const uint32_t s = sums % kDkvStages, at = s * 2 * kTile;
 #pragma unroll
-                    for (int d = 0; d < DP / 16; ++d)
-                        tc::mma(buffer + kTmemS, tc::desc_k(q + (d >> 2) * 128 * 128 + (d & 3) * 32), tc::desc_k(base + S::kKeys + (d >> 2) * 64 * 128 + (d & 3) * 32), id_s, d != 0);
+                        for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDv, q_mn + (at + kTile + r * 128), p_mn + r * 128, id_t, sums != first || r);
 #pragma unroll
-                    for (int d = 0; d < DP / 16; ++d)
-                        tc::mma(buffer + kTmemD, tc::desc_k(g + (d >> 2) * 128 * 128 + (d & 3) * 32), tc::desc_k(base + S::kValues + (d >> 2) * 64 * 128 + (d & 3) * 32), id_s, d != 0);
-                    tc::commit(&scored[tile_count & 1u]);
-                    if (j) second(k, j == 1, false);
+                        for (int r = 0; r < 8; ++r) tc::mma(tmem + kTmemDk, q_mn + (at + r * 128), d_mn + r * 128, id_t, sums != first || r);
+                        tc::commit(&empty[s]);
+                        tc::commit(used);
+                        if (++sums == end) tc::commit(summed);
+                        idle = 0;
+                    } else if (scores < end && scores < sums + 2 && ptx::mbar_test(&full[scores % kDkvStages], (scores / kDkvStages) & 1u)) {
+                        tc::fence_after();
+                        const uint32_t at = scores % kDkvStages * 2 * kTile, buffer = tmem + (scores & 1u) * kTmemBuffer;
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d) tc::mma(buffer + kTmemS, q_k + (at + (d >> 2) * 1024 + (d & 3) * 2), k_k + ((d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d) tc::mma(buffer + kTmemD, q_k + (at + kTile + (d >> 2) * 1024 + (d & 3) * 2), v_k + ((d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+                        tc::commit(&scored[scores & 1u]);
+                        ++scores;
+                        idle = 0;
+                    } else if (++idle == kPolls) {
+                        ok = false;
+                        break;
+                    }
                 }
-                if (ok) second(k, n_tiles == 1, true);
             }
             if (!ok) misc[1] = 1;
         }
