@@ -1,14 +1,10 @@
 // Attention over selected blocks, forward: out = softmax(scale q K^T) V over the visible keys of the blocks that each query names.
 //
-// Two kernels.  A tile of neighbouring queries shares the blocks that several of them name: block_attention_kernel.  A single token (or
-// few) has its blocks split over the warps of up to eight thread blocks: block_attention_split_kernel.
+// Two kernels.  A tile of neighbouring queries shares the blocks that several of them name: block_attention_kernel, on tcgen05.  A single
+// token (or few) has its blocks split over the warps of up to eight thread blocks: block_attention_split_kernel, on mma.sync.
 //
-// Both form the transposed products S^T = K Q^T and O^T = V^T P^T, so that keys and dims are the 16 rows of a tensor-core
-// instruction and (query, head) pairs its eight columns: with eight heads to a group a column tile is one query, and a query that does
-// not name a block costs nothing there.  (A tcgen05 tile of 128 rows would multiply every query of the tile with every block of the union.)
-// Softmax with a running maximum and sum per column, in fp32; P is rounded to the 16-bit type for the second product, the sum is
-// taken before that rounding.  A masked key never touches a result, whatever stands there: its score is replaced, and its value is cut out of the
-// second product's operand (0 times infinity would not be 0).
+// Softmax with a running maximum and sum per row, in fp32; P is rounded to the 16-bit type for the second product, the sum is taken before
+// that rounding.  A key that a query does not look at never touches its result, whatever stands there.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -27,12 +23,9 @@ namespace {
 
 __device__ uint32_t g_status;  // set to 1 when a bounded wait gives up
 
-constexpr int kRingBytes = 128 * 1024;  // keys and values in flight per thread block of the tile kernel
-
 // A unit of keys in shared memory: DP / 64 tiles of UNIT rows x 128 bytes (swizzled) of keys, then the same of values.
 template <int DP, int UNIT> constexpr int kHalfBytes = DP / 64 * UNIT * 128;
 template <int DP, int UNIT> constexpr int kUnitBytes = 2 * kHalfBytes<DP, UNIT>;
-template <int DP, int UNIT> constexpr int kRing = kRingBytes / kUnitBytes<DP, UNIT> < 8 ? kRingBytes / kUnitBytes<DP, UNIT> : 8;
 
 template <int DP, int UNIT>
 __device__ __forceinline__ void load_unit(unsigned char *stage, const CUtensorMap *k_map, const CUtensorMap *v_map, int kv, int row, int outer, uint64_t *bar)
@@ -131,232 +124,269 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 }
 
 // ---- a tile of queries -------------------------------------------------------------------------------------------------
-// WARPS warps of NT column tiles each, and one that loads.  The warps of a block take a unit when it has landed and leave it when they are
-// done, without waiting for each other; a unit that none of a warp's queries names is passed over.
-struct TileShape {
-    uint32_t stride, queries, chunks;  // columns of a query's heads, queries of a thread block, chunks of a group's heads
+// 128 rows -- up to 32 neighbouring queries with all heads of a group (or a chunk of them) -- against the union of the tiles of 64 keys that they name:
+//     S = Q K^T (128 x 64, two buffers in tensor memory);  P from registers back into S's columns as 16-bit operand;  O += P V.
+// Warps 0-3 hold a row each lane (a row's maximum and sum need no other lane), warp 4 loads, warp 5 multiplies whatever is ready.
+// Rows whose query does not name a tile have P = 0 there.  Multiplying only what is named, on mma.sync with a query's eight heads as the columns of
+// an instruction, was slower for every group, block size and dim tried with the blocks of a selection: 8192 queries, 32 heads, 16 blocks of 64, where
+// 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 510; 4096 queries, one head to a group, 16 blocks of 16 302 against 226.
+// The maximum is raised only when a score exceeds it by 2^8, so that O is rescaled in tensor memory a few times per row instead of once per
+// tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM: one multiplies while the other's rows are at work.
+// 0 times a value that is no number is not 0: rows of V behind the last visible key are zeroed as they land, and a row whose result is
+// not finite is formed again, key by key, from what its query looks at (exact_row).
+constexpr int kTcThreads = 192;
+constexpr int kTcStages = 2;
+constexpr uint32_t kTcO = 128, kTcCols = 256;  // columns of tensor memory: two buffers of S, O
+constexpr float kRaise = 8.f;                  // log2
+
+template <int DP> struct TcSmem {
+    static constexpr int kHalves = DP / 64;
+    static constexpr int kQ = 0;
+    static constexpr int kRing = kHalves * 128 * 128;
+    static constexpr int kStage = 2 * kHalves * 64 * 128;
+    static constexpr int kBars = kRing + kTcStages * kStage;
+    static constexpr int kLists = kBars + 128;
 };
 
-template <class T, int DP, int UNIT, int WARPS, int NT>
-__global__ void __launch_bounds__((WARPS + 1) * 32, 1) block_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttentionArgs a, TileShape shape)
+// One row by itself: a warp, four dims a lane, over the keys its query looks at.
+template <class T> __device__ void exact_row(const AttentionArgs &a, const TileUnion &u, uint32_t b, uint32_t kv, uint32_t t, uint32_t q_of_tile, uint32_t head)
 {
-    constexpr int KT = UNIT / 16, STAGES = kRing<DP, UNIT>;
+    const uint32_t lane = threadIdx.x & 31, d = lane * 4;
+    const bool on = d < a.dim;
+    const T *qr = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)t * a.q_query + (int64_t)head * a.q_head + d;
+    float q[4] = {}, o[4] = {}, top = -INFINITY, sum = 0.f;
+    if (on)
+        for (int j = 0; j < 4; ++j) q[j] = to_f32(qr[j]);
+    for (uint32_t slot = 0; slot < *u.size; ++slot)
+        for (uint64_t seen = u.seen(slot, q_of_tile, a.block); seen; seen &= seen - 1) {
+            const uint32_t key = u.tiles[slot] * kKeyTile + __ffsll((long long)seen) - 1;
+            const T *kr = key_row<T>(a, a.k, a.k_batch, a.k_key, a.k_head, b, kv, key) + d, *vr = key_row<T>(a, a.v, a.v_batch, a.v_key, a.v_head, b, kv, key) + d;
+            float s = 0.f;
+            if (on)
+                for (int j = 0; j < 4; ++j) s = fmaf(q[j], to_f32(kr[j]), s);
+#pragma unroll
+            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
+            s *= a.scale * kLog2e;
+            const float m = fmaxf(top, s), base = m == -INFINITY ? 0.f : m, f = exp2f(top - base), p = exp2f(s - base);
+            sum = sum * f + p;
+            for (int j = 0; j < 4; ++j) o[j] = o[j] * f + (on ? p * to_f32(vr[j]) : 0.f);
+            top = m;
+        }
+    const uint64_t row = ((uint64_t)b * a.queries + t) * a.heads + head;
+    if (on)
+        for (int j = 0; j < 4; ++j) static_cast<T *>(a.out)[row * a.dim + d + j] = from_f32<T>(sum != 0.f ? o[j] / sum : 0.f);
+    if (lane == 0) a.lse[((uint64_t)b * a.heads + head) * a.queries + t] = sum != 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, AttentionArgs a, TcShape shape)
+{
+    using S = TcSmem<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * kUnitBytes<DP, UNIT>), *empty = full + STAGES;
-    volatile uint32_t *gave_up = reinterpret_cast<volatile uint32_t *>(empty + STAGES);
-    BlockUnion u(reinterpret_cast<unsigned char *>(empty + STAGES + 2), shape.queries, a.count, a.num_blocks);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars), *empty = full + kTcStages, *q_full = empty + kTcStages, *scored = q_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(landed + 1);  // [0] tensor memory, [1] gave up
+    TileUnion u(smem + S::kLists, shape.queries, a);
     const uint32_t t0 = blockIdx.x * shape.queries, b = blockIdx.z;
-    const uint32_t kv = blockIdx.y / shape.chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % shape.chunks * kHeadChunk;
-    const uint32_t heads = min(kHeadChunk, group - head0), queries = min(shape.queries, a.queries - t0);
+    const uint32_t kv = blockIdx.y / shape.chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % shape.chunks * shape.heads;
+    const uint32_t heads = min(shape.heads, group - head0), queries = min(shape.queries, a.queries - t0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < kTcStages; ++s) {
             ptx::mbar_init(&full[s], 1);
-            ptx::mbar_init(&empty[s], WARPS);
+            ptx::mbar_init(&empty[s], 1);
+            ptx::mbar_init(&scored[s], 1);
+            ptx::mbar_init(&formed[s], 4);  // per buffer: a warp without work may be a tile ahead of the others
         }
-        *gave_up = 0;
+        ptx::mbar_init(q_full, 1);
+        ptx::mbar_init(summed, 1);
+        ptx::mbar_init(landed, 1);
+        misc[1] = 0;
         ptx::fence_mbar_init();
     }
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kTcCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = misc[0];
     ptx::grid_wait();
     ptx::grid_release();
-    u.build(a, b, kv, t0, queries);  // its barriers also cover the ones above
-    const uint32_t per_block = a.block / UNIT, units = *u.size * per_block;
-
-    if (warp == WARPS) {
-        if (lane == 0) {
-            uint32_t i = 0;
-            for (; i < units && !*gave_up; ++i) {
-                const uint32_t s = i % STAGES;
-                if (!ptx::mbar_wait(&empty[s], ((i / STAGES) & 1u) ^ 1u)) {
-                    *gave_up = 1;
-                    break;
-                }
-                int row, outer;
-                unit_place(a, b, u.blocks[i / per_block], i % per_block * UNIT, row, outer);
-                load_unit<DP, UNIT>(smem + s * kUnitBytes<DP, UNIT>, &k_map, &v_map, (int)kv, row, outer, &full[s]);
-            }
-            if (*gave_up) {
-                atomicExch(&g_status, 1u);
-                for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j) ptx::mbar_wait(&full[j % STAGES], (j / STAGES) & 1u);  // no copy stays in flight
-            }
-        }
-        return;
+    if (warp == 4 && lane == 0) {
+        ptx::mbar_expect_tx(q_full, S::kHalves * shape.queries * shape.heads * 128);
+        for (int h = 0; h < S::kHalves; ++h) tc::tma_load4(smem + S::kQ + h * 128 * 128, &q_map, h * 64, (int)(kv * group + head0), (int)t0, (int)b, q_full);
     }
+    u.build(a, b, kv, t0, queries);
+    const uint32_t units = *u.size;
 
-    ColumnTile<T, DP> tile[NT];
-    uint32_t asks[NT];          // the queries of a column tile, a bit each
-    uint32_t query[NT][2];      // of this lane's two columns (32: none)
-    int sees[NT][2];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const uint32_t c0 = (warp * NT + i) * 8;
-        const uint32_t c = c0 + lane / 4, ct = c / shape.stride, ch = c % shape.stride;
-        const T *row = nullptr;
-        if (ct < queries && ch < heads)
-            row = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(t0 + ct) * a.q_query + (int64_t)(kv * group + head0 + ch) * a.q_head;
-        tile[i].start(row, a.dim, lane);
-        asks[i] = 0;
-        for (uint32_t j = c0 / shape.stride; j <= (c0 + 7) / shape.stride; ++j)
-            if (j < queries && c0 - min(c0, j * shape.stride) < heads) asks[i] |= 1u << j;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t col = c0 + 2 * (lane & 3) + h, t = col / shape.stride;
-            const bool on = t < queries && col % shape.stride < heads;
-            query[i][h] = on ? t : 32u;
-            sees[i][h] = on ? (int)u.visible[t] : 0x7fffffff;
+    bool ok = true;
+    if (warp == 4) {
+        uint32_t phase = 0, i = 0;
+        for (; i < units; ++i) {
+            const uint32_t s = i % kTcStages;
+            if (!(ok = ptx::mbar_wait_warp(&empty[s], ((i / kTcStages) & 1u) ^ 1u))) break;
+            if (!(ok = load_key_tile<DP>(smem + S::kRing + s * S::kStage, &k_map, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase))) break;
         }
-    }
-    const float scale_log2 = a.scale * kLog2e;
-
-    for (uint32_t n = 0; n < units; ++n) {
-        const uint32_t s = n % STAGES, slot = n / per_block, names = u.names[slot];
-        const int first = (int)(u.blocks[slot] * a.block + n % per_block * UNIT);
-        if (!ptx::mbar_wait(&full[s], (n / STAGES) & 1u)) {
-            *gave_up = 1;
-            if (lane == 0) atomicExch(&g_status, 1u);
-            return;
+        if (!ok) {
+            misc[1] = 1;
+            if (lane == 0) {  // no copy stays in flight
+                ptx::mbar_wait(q_full, 0);
+                for (uint32_t j = i > kTcStages ? i - kTcStages : 0; j < i; ++j) ptx::mbar_wait(&full[j % kTcStages], (j / kTcStages) & 1u);
+            }
+        } else if (!units && lane == 0)
+            ok = ptx::mbar_wait(q_full, 0);
+    } else if (warp == 5) {
+        if (lane == 0 && units) {
+            constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+            constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_o = tc::idesc(bf16, 128, DP, false, true);
+            const uint32_t base = ptx::smem_u32(smem);
+            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), v_mn = tc::desc_mn(base + S::kRing + S::kHalves * 64 * 128, 64 * 128);
+            ok = ptx::mbar_wait(q_full, 0);
+            uint32_t scores = 0, sums = 0;
+            for (uint32_t idle = 0; ok && sums < units;) {
+                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u)) {
+                    tc::fence_after();
+                    const uint32_t s = sums % kTcStages, at = s * (S::kStage >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kTcO, tmem + (sums & 1u) * 64 + k * 8, v_mn + (at + k * 128), id_o, sums || k);
+                    tc::commit(&empty[s]);
+                    tc::commit(summed);
+                    ++sums;
+                    idle = 0;
+                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&full[scores % kTcStages], (scores / kTcStages) & 1u)) {
+                    tc::fence_after();
+                    const uint32_t at = scores % kTcStages * (S::kStage >> 4);
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d) tc::mma(tmem + (scores & 1u) * 64, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+                    tc::commit(&scored[scores & 1u]);
+                    ++scores;
+                    idle = 0;
+                } else if (++idle == kTcPolls)
+                    ok = false;
+            }
+            if (!ok) misc[1] = 1;
         }
-        bool on[NT], any = false;
+    } else {
+        const uint32_t r = threadIdx.x, q = r / shape.heads, h = r % shape.heads, head = kv * group + head0 + h;
+        const bool real = q < queries && h < heads;
+        const uint32_t lanes = tmem + ((warp * 32) << 16);
+        const float scale_log2 = a.scale * kLog2e;
+        float top = -INFINITY, sum = 0.f;
+        for (uint32_t i = 0; i < units; ++i) {
+            const uint64_t seen = real ? u.seen(i, q, a.block) : 0ull;
+            const uint32_t buffer = lanes + (i & 1u) * 64;
+            if (!(ok = ptx::mbar_wait_warp(&scored[i & 1u], (i >> 1) & 1u))) break;
+            tc::fence_after();
+            uint32_t p[32];
+            if (__any_sync(~0u, seen != 0)) {
+                uint32_t v[64];
+                tc::ld32(buffer, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                tc::ld32(buffer + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+                tc::wait_ld();
+                const bool plain = __all_sync(~0u, seen == 0 || seen == ~0ull);
+                if (!plain) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) any |= on[i] = (names & asks[i]) != 0;
-        if (any) {
-            const uint32_t keys = ptx::smem_u32(smem + s * kUnitBytes<DP, UNIT>), values = keys + kHalfBytes<DP, UNIT>;
-            float sc[NT][KT][4];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int k = 0; k < KT; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[i][k][j] = 0.f;
-#pragma unroll
-            for (int k = 0; k < KT; ++k)
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    uint32_t f[4];
-                    tc::ldmatrix4(f, keys_at(keys, UNIT, k, d, lane));
-#pragma unroll
-                    for (int i = 0; i < NT; ++i)
-                        if (on[i]) tc::mma16<T>(sc[i][k], f, tile[i].q[d][0], tile[i].q[d][1]);
+                    for (int c = 0; c < 64; ++c)
+                        if (!((uint32_t)(seen >> (c & 32)) & (1u << (c & 31)))) v[c] = 0xff800000u;
                 }
-            uint32_t p[NT][KT][2];
-            bool whole[NT], slow = false;
-            int limit[NT][2];
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains: one of 64 would be the latency of 64 instructions
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                whole[i] = true;
-                if (!on[i]) continue;
+                for (int c = 0; c < 64; c += 8)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) limit[i][h] = query[i][h] == 32u ? UNIT : (names >> query[i][h]) & 1u ? sees[i][h] - first : 0;
-                whole[i] = __all_sync(~0u, limit[i][0] >= UNIT && limit[i][1] >= UNIT);
-                if (!whole[i]) {
-                    slow = true;
-                    const int r = (int)(lane >> 2);
-#pragma unroll
-                    for (int k = 0; k < KT; ++k) {
-                        if (k * 16 + r >= limit[i][0]) sc[i][k][0] = -INFINITY;
-                        if (k * 16 + r >= limit[i][1]) sc[i][k][1] = -INFINITY;
-                        if (k * 16 + r + 8 >= limit[i][0]) sc[i][k][2] = -INFINITY;
-                        if (k * 16 + r + 8 >= limit[i][1]) sc[i][k][3] = -INFINITY;
+                    for (int x = 0; x < 4; ++x) m4[x] = ptx::max3(m4[x], __uint_as_float(v[c + 2 * x]), __uint_as_float(v[c + 2 * x + 1]));
+                float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                m *= scale_log2;
+                bool raise = false;
+                float f = 1.f;
+                if (seen) {
+                    if (top == -INFINITY) top = m;  // nothing summed yet
+                    else if (m > top + kRaise) {
+                        raise = true;
+                        f = tc::exp2_fast(top - m);
+                        top = m;
+                        sum *= f;
                     }
                 }
-                tile[i].softmax(sc[i], p[i], scale_log2);
-            }
-            if (!slow) {
+                if (__any_sync(~0u, raise)) {
+                    if (!(ok = ptx::mbar_wait_warp(summed, (i - 1) & 1u))) break;  // the products in flight add to O
+                    tc::fence_after();
+#pragma unroll 1
+                    for (uint32_t c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tc::ld32(lanes + kTcO + c, o);
+                        tc::wait_ld();
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                    for (int k = 0; k < KT; ++k) {
-                        uint32_t f[4];
-                        tc::ldmatrix4_trans(f, values_at(values, UNIT, k, d, lane));
-#pragma unroll
-                        for (int i = 0; i < NT; ++i)
-                            if (on[i]) tc::mma16<T>(tile[i].o[d], f, p[i][k][0], p[i][k][1]);
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tc::st32(lanes + kTcO + c, o);
                     }
+                }
+                // a row that does not name the tile: every exponential is 0 (a score that is no number makes its result none, and that is formed again)
+                const float minus = !seen ? -INFINITY : top == -INFINITY ? 0.f : -top;
+                const uint64_t scale2 = ptx::pack2(scale_log2, scale_log2), minus2 = ptx::pack2(minus, minus);
+                uint64_t part[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    const float2 x = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), scale2, minus2));
+                    const float e0 = tc::exp2_fast(x.x), e1 = tc::exp2_fast(x.y);
+                    part[c & 1] = ptx::add2(part[c & 1], ptx::pack2(e0, e1));
+                    p[c] = tc::round2<T>(e0, e1);
+                }
+                const float2 both = ptx::unpack2(ptx::add2(part[0], part[1]));
+                sum += both.x + both.y;
+                __syncwarp();
             } else {
-                // Queries of one column tile that see different parts of the unit: a pass for those that see all of it, one for each
-                // other; a pass changes its own columns only.
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    if (!on[i]) continue;
-                    uint32_t left = names & asks[i];
-                    bool all = true;  // first the pass over whole units
-                    while (left) {
-                        int cut = UNIT;
-                        uint32_t taken = 0;
-                        if (all) {
-                            for (uint32_t m = left; m; m &= m - 1) {
-                                const uint32_t t = __ffs(m) - 1;
-                                if ((int)u.visible[t] - first >= UNIT) taken |= 1u << t;
-                            }
-                            all = false;
-                        } else {
-                            const uint32_t t = __ffs(left) - 1;
-                            taken = 1u << t;
-                            cut = (int)u.visible[t] - first;
-                        }
-                        left &= ~taken;
-                        if (!taken || cut <= 0) continue;
-                        const bool mine0 = (taken >> query[i][0]) & (query[i][0] < 32u), mine1 = (taken >> query[i][1]) & (query[i][1] < 32u);
+                for (int c = 0; c < 32; ++c) p[c] = 0;
+            }
+            tc::st32(buffer, p);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&formed[i & 1u]);
+        }
+        // the last two, in order: a parity names the one before the last as well as the one to come
+        if (ok && units > 1) ok = ptx::mbar_wait_warp(summed, (units - 2) & 1u);
+        if (ok && units) ok = ptx::mbar_wait_warp(summed, (units - 1) & 1u);
+        tc::fence_after();
+        if (!ok) misc[1] = 1;
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        T *row = static_cast<T *>(a.out) + (((uint64_t)b * a.queries + t0 + q) * a.heads + head) * a.dim;
+        bool finite = sum < INFINITY;
+#pragma unroll 1
+        for (uint32_t c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            if (units) {
+                tc::ld32(lanes + kTcO + c, o);
+                tc::wait_ld();
+            }
 #pragma unroll
-                        for (int d = 0; d < DP / 16; ++d) {
-                            float o[4] = {tile[i].o[d][0], tile[i].o[d][1], tile[i].o[d][2], tile[i].o[d][3]};
+            for (int x = 0; x < 4; ++x) {
+                uint32_t w[4];
 #pragma unroll
-                            for (int k = 0; k < KT; ++k) {
-                                uint32_t f[4];
-                                tc::ldmatrix4_trans(f, values_at(values, UNIT, k, d, lane));
-                                if (cut < UNIT) {
-                                    const int at = k * 16 + 2 * (int)(lane & 3);
-                                    f[0] = keep_keys(f[0], at, cut);
-                                    f[1] = keep_keys(f[1], at, cut);
-                                    f[2] = keep_keys(f[2], at + 8, cut);
-                                    f[3] = keep_keys(f[3], at + 8, cut);
-                                }
-                                tc::mma16<T>(o, f, p[i][k][0], p[i][k][1]);
-                            }
-                            if (mine0) {
-                                tile[i].o[d][0] = o[0];
-                                tile[i].o[d][2] = o[2];
-                            }
-                            if (mine1) {
-                                tile[i].o[d][1] = o[1];
-                                tile[i].o[d][3] = o[3];
-                            }
-                        }
-                    }
+                for (int y = 0; y < 4; ++y) {
+                    const float o0 = units ? __uint_as_float(o[8 * x + 2 * y]) : 0.f, o1 = units ? __uint_as_float(o[8 * x + 2 * y + 1]) : 0.f;
+                    finite = finite && fabsf(o0) < INFINITY && fabsf(o1) < INFINITY;
+                    w[y] = tc::round2<T>(o0 * inv, o1 * inv);
                 }
+                if (real && c + 8 * x < a.dim) *reinterpret_cast<uint4 *>(row + c + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&empty[s]);
+        if (real) a.lse[((uint64_t)b * a.heads + head) * a.queries + t0 + q] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        for (uint32_t left = __ballot_sync(~0u, real && !finite); left && !misc[1]; left &= left - 1) {
+            const uint32_t from = __ffs(left) - 1, rq = __shfl_sync(~0u, q, from), rh = __shfl_sync(~0u, head, from);
+            __syncwarp();
+            exact_row<T>(a, u, b, kv, t0 + rq, rq, rh);
+        }
     }
-
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        tile[i].finish_sum();
-        const float f0 = tile[i].sum[0] > 0.f ? 1.f / tile[i].sum[0] : 0.f, f1 = tile[i].sum[1] > 0.f ? 1.f / tile[i].sum[1] : 0.f;
-        const uint32_t c = (warp * NT + i) * 8 + lane / 4, t = c / shape.stride, h = c % shape.stride;
-        const bool row_on = t < queries && h < heads;
-        T *row = static_cast<T *>(a.out) + (((uint64_t)b * a.queries + t0 + t) * a.heads + kv * group + head0 + h) * a.dim;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            const uint32_t lo = tc::transpose8x8(tc::round2<T>(tile[i].o[d][0] * f0, tile[i].o[d][1] * f1));
-            const uint32_t hi = tc::transpose8x8(tc::round2<T>(tile[i].o[d][2] * f0, tile[i].o[d][3] * f1));
-            const uint32_t at = d * 16 + 2 * (lane & 3);
-            if (row_on && at < a.dim) *reinterpret_cast<uint32_t *>(row + at) = lo;
-            if (row_on && at + 8 < a.dim) *reinterpret_cast<uint32_t *>(row + at + 8) = hi;
-        }
-        if (lane < 4)
-#pragma unroll
-            for (int h2 = 0; h2 < 2; ++h2) {
-                const uint32_t col = (warp * NT + i) * 8 + 2 * lane + h2, ct = col / shape.stride, ch = col % shape.stride;
-                if (ct < queries && ch < heads)
-                    a.lse[((uint64_t)b * a.heads + kv * group + head0 + ch) * a.queries + t0 + ct] =
-                        tile[i].sum[h2] > 0.f ? (tile[i].top[h2] + log2f(tile[i].sum[h2])) * 0.6931471805599453f : -INFINITY;
-            }
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && misc[1]) atomicExch(&g_status, 1u);
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tmem, kTcCols);
     }
 }
 
 // ---- a single token ----------------------------------------------------------------------------------------------------
+// The products are formed transposed, S^T = K Q^T and O^T = V^T P^T: keys and dims are the 16 rows of an instruction and the group's heads its eight columns.
 // One query's heads of one head of keys: its blocks, in pieces of 16 keys, are dealt over the warps of a cluster of thread blocks.  A
 // warp fills a ring of its own (its lane 0 issues the loads) and keeps its own softmax state; the states are joined in the
 // order of the warps, first inside a thread block, then over the cluster through distributed shared memory: no scratch, no counters, one
@@ -459,7 +489,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
     const float scale_log2 = a.scale * kLog2e;
     for (uint32_t i = 0; i < mine_units; ++i) {
         const uint32_t n = me + i * walkers, s = i % STAGES;
-        if (!ptx::mbar_wait(&full[s], (i / STAGES) & 1u)) {  // later loads of this ring land before the block ends, or their waits give up too
+        if (!ptx::mbar_wait_warp(&full[s], (i / STAGES) & 1u)) {  // later loads of this ring land before the block ends, or their waits give up too
             if (lane == 0) atomicExch(&g_status, 1u);
             continue;
         }
@@ -583,37 +613,24 @@ template <class T, int DP, int NT> cudaError_t launch_split(const CUtensorMap &k
     return cudaLaunchKernelEx(&cfg, block_attention_split_kernel<T, DP, NT>, k_map, v_map, a, chunks);
 }
 
-template <class T, int DP, int UNIT, int WARPS, int NT>
-cudaError_t launch_tile(const CUtensorMap &k_map, const CUtensorMap &v_map, const AttentionArgs &a, cudaStream_t s)
+template <class T, int DP> cudaError_t launch_tile(const CUtensorMap &k_map, const CUtensorMap &v_map, const AttentionArgs &a, uint32_t box_rows, cudaStream_t s)
 {
-    const uint32_t group = a.heads / a.kv_heads, heads = group < kHeadChunk ? group : kHeadChunk;
-    TileShape shape;
-    shape.stride = column_stride(heads);
-    shape.queries = WARPS * NT * 8 / shape.stride;
-    if (shape.queries > kTileQueries) shape.queries = kTileQueries;
-    shape.chunks = (group + kHeadChunk - 1) / kHeadChunk;
-    constexpr int kFixed = kRing<DP, UNIT> * (kUnitBytes<DP, UNIT> + 16) + 16;
-    const uint32_t bytes = kFixed + BlockUnion::bytes(shape.queries, a.count, a.num_blocks);
-    cudaError_t e = allow_dynamic_smem<block_attention_kernel<T, DP, UNIT, WARPS, NT>>(227 * 1024);
+    TcShape shape = tc_shape(a.heads / a.kv_heads, box_rows);
+    uint32_t bytes = 0;  // fewer queries where their lists are too long (more than 100 blocks of 16 for each of 32 queries)
+    for (;; shape.queries /= 2)
+        if ((bytes = TcSmem<DP>::kLists + TileUnion::bytes(shape.queries, a.count, a.block, a.keys)) <= kSmemMost || shape.queries == 1) break;
+    CUtensorMap q_map;
+    cudaError_t e = tc::make_map(&q_map, std::is_same<T, __nv_bfloat16>::value, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, shape.queries, shape.heads);
+    if (e == cudaSuccess) e = allow_dynamic_smem<block_attention_kernel<T, DP>>(kSmemMost);
     if (e != cudaSuccess) return e;
     const dim3 grid((a.queries + shape.queries - 1) / shape.queries, a.kv_heads * shape.chunks, a.batch);
-    return launch_overlapped(block_attention_kernel<T, DP, UNIT, WARPS, NT>, grid, dim3((WARPS + 1) * 32), bytes, s, k_map, v_map, a, shape);
+    return launch_overlapped(block_attention_kernel<T, DP>, grid, dim3(kTcThreads), bytes, s, k_map, v_map, q_map, a, shape);
 }
 
-template <class T, int DP> cudaError_t launch_d(const CUtensorMap &k_map, const CUtensorMap &v_map, const AttentionArgs &a, bool split, int sm_count, cudaStream_t s)
+template <class T, int DP> cudaError_t launch_d(const CUtensorMap &k_map, const CUtensorMap &v_map, const AttentionArgs &a, bool split, uint32_t box_rows, int sm_count, cudaStream_t s)
 {
-    const uint32_t group = a.heads / a.kv_heads;
-    if (split) return group <= 8 ? launch_split<T, DP, 1>(k_map, v_map, a, sm_count, s) : launch_split<T, DP, 2>(k_map, v_map, a, sm_count, s);
-    auto unit = [&](auto u) {
-        constexpr int U = decltype(u)::value;
-        // a tile has at most 32 queries: groups of one or two heads fill fewer columns
-        if (group == 1) return launch_tile<T, DP, U, 4, 1>(k_map, v_map, a, s);
-        if (group == 2) return launch_tile<T, DP, U, 4, 2>(k_map, v_map, a, s);
-        return launch_tile<T, DP, U, 8, 2>(k_map, v_map, a, s);
-    };
-    if (a.block == 16) return unit(std::integral_constant<int, 16>());
-    if (a.block == 32) return unit(std::integral_constant<int, 32>());
-    return unit(std::integral_constant<int, 64>());
+    if (!split) return launch_tile<T, DP>(k_map, v_map, a, box_rows, s);
+    return a.heads / a.kv_heads <= 8 ? launch_split<T, DP, 1>(k_map, v_map, a, sm_count, s) : launch_split<T, DP, 2>(k_map, v_map, a, sm_count, s);
 }
 
 }  // namespace
@@ -625,7 +642,7 @@ cudaError_t launch_block_attention(const AttentionArgs &a, int sm_count, cudaStr
     // few queries: a thread block per query and head of keys, its blocks split over warps
     const bool split = a.queries <= 4;
     const uint32_t rows = a.pages ? a.block : a.keys, outer = a.pages ? a.num_pages : a.batch;
-    const uint32_t box = split ? (uint32_t)kSplitUnit : a.block < 64 ? a.block : 64;
+    const uint32_t box = split ? (uint32_t)kSplitUnit : a.pages && a.block < 64 ? a.block : 64u;
     CUtensorMap k_map{}, v_map{};
     if (rows && outer) {  // without keys no block counts and nothing is loaded
         cudaError_t e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, rows, outer, a.k_head, a.k_key, a.k_batch, box);
@@ -633,8 +650,8 @@ cudaError_t launch_block_attention(const AttentionArgs &a, int sm_count, cudaStr
         if (e != cudaSuccess) return e;
     }
     if (bf16)
-        return a.dim <= 64 ? launch_d<__nv_bfloat16, 64>(k_map, v_map, a, split, sm_count, s) : launch_d<__nv_bfloat16, 128>(k_map, v_map, a, split, sm_count, s);
-    return a.dim <= 64 ? launch_d<__half, 64>(k_map, v_map, a, split, sm_count, s) : launch_d<__half, 128>(k_map, v_map, a, split, sm_count, s);
+        return a.dim <= 64 ? launch_d<__nv_bfloat16, 64>(k_map, v_map, a, split, box, sm_count, s) : launch_d<__nv_bfloat16, 128>(k_map, v_map, a, split, box, sm_count, s);
+    return a.dim <= 64 ? launch_d<__half, 64>(k_map, v_map, a, split, box, sm_count, s) : launch_d<__half, 128>(k_map, v_map, a, split, box, sm_count, s);
 }
 
 cudaError_t block_attention_status(uint32_t *word) { return read_status(g_status, word); }

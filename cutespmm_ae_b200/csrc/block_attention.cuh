@@ -13,6 +13,7 @@
 namespace cutespmm {
 
 constexpr uint32_t kTileQueries = 32;  // at most: a bit of a word each
+constexpr uint32_t kHeadChunk = 64;    // query heads of a group that one block of threads takes, at most
 constexpr float kLog2e = 1.4426950408889634f;
 
 // How many keys query t of sequence b sees.
@@ -30,76 +31,7 @@ __device__ __forceinline__ bool block_counts(const AttentionArgs &a, uint32_t b,
     return page >= 0 && (uint32_t)page < a.num_pages;
 }
 
-// The union of the blocks that `queries` queries from t0 on name, ascending, each with a bit per query that names it.
-struct BlockUnion {
-    uint32_t *blocks, *names;  // up to kTileQueries * count
-    uint32_t *visible;         // per query of the tile
-    uint32_t *bits, *before;   // a bit per block of the sequence, and the blocks in front of each word
-    uint32_t *size;
-
-    static __host__ __device__ uint32_t words(uint32_t num_blocks) { return (num_blocks + 31) / 32; }
-    static __host__ __device__ uint32_t slots(uint32_t queries, uint32_t count, uint32_t num_blocks)
-    {
-        const uint32_t n = queries * count;
-        return n < num_blocks ? n : num_blocks;
-    }
-    static __host__ __device__ uint32_t bytes(uint32_t queries, uint32_t count, uint32_t num_blocks)
-    {
-        return (2 * slots(queries, count, num_blocks) + kTileQueries + 2 * words(num_blocks) + 4) * 4;
-    }
-    __device__ BlockUnion(unsigned char *p, uint32_t queries, uint32_t count, uint32_t num_blocks)
-    {
-        uint32_t *w = reinterpret_cast<uint32_t *>(p);
-        size = w;
-        visible = w + 4;
-        bits = visible + kTileQueries;
-        before = bits + words(num_blocks);
-        blocks = before + words(num_blocks);
-        names = blocks + slots(queries, count, num_blocks);
-    }
-    // every thread of the block; ends with a barrier
-    __device__ void build(const AttentionArgs &a, uint32_t b, uint32_t kv, uint32_t t0, uint32_t queries)
-    {
-        const uint32_t w = words(a.num_blocks), n = queries * a.count;
-        const int32_t *src = a.blocks + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0) * a.count;
-        for (uint32_t i = threadIdx.x; i < w; i += blockDim.x) bits[i] = 0;
-        for (uint32_t i = threadIdx.x; i < queries; i += blockDim.x) visible[i] = visible_keys(a, b, t0 + i);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const int32_t j = src[i];
-            if (block_counts(a, b, j, visible[i / a.count])) atomicOr(&bits[j >> 5], 1u << (j & 31));
-        }
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            uint32_t sum = 0;
-            for (uint32_t i = 0; i < w; i += 32) {
-                const uint32_t mine = i + threadIdx.x < w ? __popc(bits[i + threadIdx.x]) : 0u;
-                uint32_t scan = mine;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const uint32_t up = __shfl_up_sync(~0u, scan, d);
-                    if (threadIdx.x >= (uint32_t)d) scan += up;
-                }
-                if (i + threadIdx.x < w) before[i + threadIdx.x] = sum + scan - mine;
-                sum += __shfl_sync(~0u, scan, 31);
-            }
-            if (threadIdx.x == 0) *size = sum;
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < *size; i += blockDim.x) names[i] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const int32_t j = src[i];
-            if (!block_counts(a, b, j, visible[i / a.count])) continue;
-            const uint32_t at = before[j >> 5] + __popc(bits[j >> 5] & ((1u << (j & 31)) - 1u));
-            blocks[at] = (uint32_t)j;
-            atomicOr(&names[at], 1u << (i / a.count));
-        }
-        __syncthreads();
-    }
-};
-
-// Where unit `sub` (of `unit` keys) of block j of sequence b lies: coordinates of the tensor maps over k and v.
+// Where the keys from the `first`-th of block j of sequence b on lie: coordinates of the tensor maps over k and v.
 __device__ __forceinline__ void unit_place(const AttentionArgs &a, uint32_t b, uint32_t j, uint32_t first, int &row, int &outer)
 {
     if (a.pages) {
@@ -111,10 +43,167 @@ __device__ __forceinline__ void unit_place(const AttentionArgs &a, uint32_t b, u
     }
 }
 
-// Columns: the products are formed transposed, keys (then dims) as rows and (query, head) pairs as columns, eight columns to a
-// tensor-core tile.  The heads of a group take `stride` columns: 1, 2, 4 or a multiple of 8.
-__host__ __device__ inline uint32_t column_stride(uint32_t heads) { return heads <= 1 ? 1 : heads <= 2 ? 2 : heads <= 4 ? 4 : (heads + 7) / 8 * 8; }
-constexpr uint32_t kHeadChunk = 64;  // query heads of a group that one block of threads takes
+// ---- tiles of 64 keys ----------------------------------------------------------------------------------------------------
+// The tcgen05 kernels walk keys 64 at a time whatever the blocks are: a block of 128 is two tiles, four blocks of 16 are one.
+constexpr uint32_t kKeyTile = 64;
+__host__ __device__ inline uint32_t parts_of_tile(uint32_t block) { return block < kKeyTile ? kKeyTile / block : 1; }
+__host__ __device__ inline uint32_t tiles_of_block(uint32_t block) { return block > kKeyTile ? block / kKeyTile : 1; }
+
+// The union of the tiles of keys that hold a block which some of `queries` queries from t0 on name, ascending; for each part (block) of
+// each tile a bit per query that names it.
+struct TileUnion {
+    uint32_t *tiles, *names;  // names: slot * parts + part
+    uint32_t *visible, *bits, *before, *size;
+    uint32_t parts;
+
+    static __host__ __device__ uint32_t words(uint32_t keys) { return (keys + kKeyTile * 32 - 1) / (kKeyTile * 32); }
+    static __host__ __device__ uint32_t slots(uint32_t queries, uint32_t count, uint32_t block, uint32_t keys)
+    {
+        const uint32_t n = queries * count * tiles_of_block(block), all = (keys + kKeyTile - 1) / kKeyTile;
+        return n < all ? n : all;
+    }
+    static __host__ __device__ uint32_t bytes(uint32_t queries, uint32_t count, uint32_t block, uint32_t keys)
+    {
+        return (slots(queries, count, block, keys) * (1 + parts_of_tile(block)) + kTileQueries + 2 * words(keys) + 4) * 4;
+    }
+    __device__ TileUnion(unsigned char *p, uint32_t queries, const AttentionArgs &a)
+    {
+        uint32_t *w = reinterpret_cast<uint32_t *>(p);
+        parts = parts_of_tile(a.block);
+        size = w;
+        visible = w + 4;
+        bits = visible + kTileQueries;
+        before = bits + words(a.keys);
+        tiles = before + words(a.keys);
+        names = tiles + slots(queries, a.count, a.block, a.keys);
+    }
+    // every thread of the block; ends with a barrier.  size[1]: the most keys that one of the queries sees
+    __device__ void build(const AttentionArgs &a, uint32_t b, uint32_t kv, uint32_t t0, uint32_t queries)
+    {
+        const uint32_t w = words(a.keys), n = queries * a.count, per = tiles_of_block(a.block);
+        const int32_t *src = a.blocks + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0) * a.count;
+        for (uint32_t i = threadIdx.x; i < w; i += blockDim.x) bits[i] = 0;
+        for (uint32_t i = threadIdx.x; i < queries; i += blockDim.x) visible[i] = visible_keys(a, b, t0 + i);
+        __syncthreads();
+        auto each = [&](auto &&fn) {  // fn(tile, part, query) for what every query names and sees a part of
+            for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+                const uint32_t q = i / a.count;
+                const int32_t j = src[i];
+                if (!block_counts(a, b, j, visible[q])) continue;
+                const uint64_t first = (uint64_t)j * a.block;
+                for (uint32_t x = 0; x < per; ++x)
+                    if (first + x * kKeyTile < visible[q]) fn((uint32_t)(first / kKeyTile) + x, (uint32_t)(first % kKeyTile) / a.block, q);
+            }
+        };
+        each([&](uint32_t tile, uint32_t, uint32_t) { atomicOr(&bits[tile >> 5], 1u << (tile & 31)); });
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            uint32_t sum = 0, most = 0;
+            for (uint32_t i = 0; i < w; i += 32) {
+                const uint32_t mine = i + threadIdx.x < w ? __popc(bits[i + threadIdx.x]) : 0u;
+                uint32_t scan = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(~0u, scan, d);
+                    if (threadIdx.x >= (uint32_t)d) scan += up;
+                }
+                if (i + threadIdx.x < w) before[i + threadIdx.x] = sum + scan - mine;
+                sum += __shfl_sync(~0u, scan, 31);
+            }
+            if (threadIdx.x < queries) most = visible[threadIdx.x];
+            most = __reduce_max_sync(~0u, most);
+            if (threadIdx.x == 0) {
+                size[0] = sum;
+                size[1] = most;
+            }
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < size[0] * parts; i += blockDim.x) names[i] = 0;
+        __syncthreads();
+        each([&](uint32_t tile, uint32_t part, uint32_t q) {
+            const uint32_t at = before[tile >> 5] + __popc(bits[tile >> 5] & ((1u << (tile & 31)) - 1u));
+            tiles[at] = tile;
+            atomicOr(&names[at * parts + part], 1u << q);
+        });
+        __syncthreads();
+    }
+    // the keys of a tile that query q looks at, a bit each
+    __device__ uint64_t seen(uint32_t slot, uint32_t q, uint32_t block) const
+    {
+        const int64_t limit = (int64_t)visible[q] - (int64_t)tiles[slot] * kKeyTile;
+        const uint64_t below = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1ull : 0ull;
+        if (parts == 1) return (names[slot] >> q) & 1u ? below : 0ull;
+        uint64_t named = 0;
+        for (uint32_t i = 0; i < parts; ++i)
+            if ((names[slot * parts + i] >> q) & 1u) named |= ((1ull << block) - 1ull) << (i * block);
+        return named & below;
+    }
+};
+
+// What a thread block of the tcgen05 kernels that walk queries takes: 128 rows, (query, head of the group) pairs.
+struct TcShape {
+    uint32_t heads, queries, chunks, box_rows;  // rows of a query, queries of a tile, chunks of a group's heads, rows of a box of k and v
+};
+inline TcShape tc_shape(uint32_t group, uint32_t box_rows)
+{
+    TcShape s;
+    s.heads = group < kHeadChunk ? group : kHeadChunk;
+    s.queries = 128 / s.heads < kTileQueries ? 128 / s.heads : kTileQueries;
+    s.chunks = (group + s.heads - 1) / s.heads;
+    s.box_rows = box_rows;
+    return s;
+}
+constexpr uint32_t kSmemMost = 227 * 1024;
+constexpr uint32_t kTcPolls = 1u << 24;  // of a role that looks at two barriers in turn, before it gives up
+
+// One warp brings the keys and values of a tile into shared memory: per operand DP / 64 tiles of 64 rows x 128 bytes, swizzled.  Rows
+// that none of the queries sees become zeros: whatever a cache holds behind the last key, 0 times it has to be 0.  box_rows: rows of a
+// box of the maps (64, or the size of a page).  Returns false when a wait gave up.
+template <int DP>
+__device__ __forceinline__ bool load_key_tile(unsigned char *stage, const CUtensorMap *k_map, const CUtensorMap *v_map, const AttentionArgs &a, uint32_t b, uint32_t kv, uint32_t tile,
+                                              uint32_t visible, uint32_t box_rows, uint64_t *full, uint64_t *landed, uint32_t &landed_phase)
+{
+    constexpr uint32_t kOperand = DP / 64 * kKeyTile * 128;
+    const uint32_t lane = threadIdx.x & 31, first = tile * kKeyTile;
+    const bool cut = first + kKeyTile > visible;
+    uint64_t *bar = cut ? landed : full;
+    if (lane == 0) {
+        ptx::mbar_expect_tx(bar, 2 * kOperand);
+        for (uint32_t r = 0; r < kKeyTile; r += box_rows) {
+            int row = (int)(first + r), outer = (int)b;
+            if (a.pages) {
+                const uint32_t j = (first + r) / a.block;
+                row = (int)((first + r) % a.block);
+                outer = j < a.page_cols ? a.pages[(uint64_t)b * a.page_cols + j] : -1;  // what is no page arrives as zeros
+            }
+#pragma unroll
+            for (int h = 0; h < DP / 64; ++h) {
+                tc::tma_load4(stage + h * kKeyTile * 128 + r * 128, k_map, h * 64, (int)kv, row, outer, bar);
+                tc::tma_load4(stage + kOperand + h * kKeyTile * 128 + r * 128, v_map, h * 64, (int)kv, row, outer, bar);
+            }
+        }
+    }
+    __syncwarp();
+    if (!cut) return true;
+    const bool ok = ptx::mbar_wait_warp(landed, landed_phase);
+    landed_phase ^= 1u;
+    const uint32_t from = visible > first ? visible - first : 0u;
+    for (uint32_t i = lane; i < 2 * (DP / 64) * (kKeyTile - from) * 8; i += 32) {
+        const uint32_t operand = i / ((kKeyTile - from) * 8), row = from + i % ((kKeyTile - from) * 8) / 8;
+        *reinterpret_cast<uint4 *>(stage + operand * kKeyTile * 128 + row * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+    }
+    ptx::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(full);
+    return ok;
+}
+
+template <class T> __device__ __forceinline__ const T *key_row(const AttentionArgs &a, const void *base, int64_t s_batch, int64_t s_key, int64_t s_head, uint32_t b, uint32_t kv, uint32_t key)
+{
+    const T *p = static_cast<const T *>(base) + (int64_t)kv * s_head;
+    if (!a.pages) return p + (int64_t)b * s_batch + (int64_t)key * s_key;
+    return p + (int64_t)a.pages[(uint64_t)b * a.page_cols + key / a.block] * s_batch + (int64_t)(key % a.block) * s_key;
+}
 
 // masks the 16-bit pair of keys k, k + 1 in a register: only keys below `limit` stay
 __device__ __forceinline__ uint32_t keep_keys(uint32_t pair, int k, int limit)

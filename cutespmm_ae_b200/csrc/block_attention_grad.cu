@@ -25,222 +25,256 @@ namespace {
 __device__ uint32_t g_status;  // set to 1 (dq) or 2 (dk, dv) when a bounded wait gives up
 
 // ---- dq ----------------------------------------------------------------------------------------------------------------
-// The forward kernel's tile and ring; a warp has one tile of eight columns, with q, dout and dq of it in registers, and takes a unit 16
-// keys at a time.  A masked key's dS is zero whatever K and V hold there, and its K is cut out of the product with dS.
-constexpr int kDqWarps = 8;
-constexpr int kDqRingBytes = 64 * 1024;
-template <int DP, int UNIT> constexpr int kDqHalf = DP / 64 * UNIT * 128;
-template <int DP, int UNIT> constexpr int kDqUnit = 2 * kDqHalf<DP, UNIT>;
-template <int DP, int UNIT> constexpr int kDqRing = kDqRingBytes / kDqUnit<DP, UNIT> < 8 ? kDqRingBytes / kDqUnit<DP, UNIT> : 8;
+// The forward kernel's 128 rows and union of key tiles.  Per tile S = Q K^T and D = dO V^T (128 x 64, two buffers of tensor memory), dS from
+// registers into tensor memory as 16-bit operand, dQ += dS K with the same bytes of K.  Eight warps form dS: a row's lse and delta are one
+// value each for the whole kernel, two threads share a row.  A row whose dq is not finite is formed again from what its query looks at.
+constexpr int kDqtWarps = 8, kDqtThreads = (kDqtWarps + 2) * 32, kDqtStages = 3;
+constexpr uint32_t kDqtBuffer = 128, kDqtSum = 256, kDqtDs = 384, kDqtCols = 512;
 
-template <class T, int DP, int UNIT>
-__global__ void __launch_bounds__((kDqWarps + 1) * 32, 2) block_attention_dq_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttentionArgs a, uint32_t stride, uint32_t tile_queries, uint32_t chunks)
+template <int DP> struct DqtSmem {
+    static constexpr int kHalves = DP / 64;
+    static constexpr int kQ = 0, kDo = kHalves * 128 * 128;
+    static constexpr int kRing = 2 * kHalves * 128 * 128;
+    static constexpr int kStage = 2 * kHalves * 64 * 128;
+    static constexpr int kDelta = kRing + kDqtStages * kStage;  // two shares of delta per row
+    static constexpr int kBars = kDelta + 2 * 128 * 4;
+    static constexpr int kLists = kBars + 128;
+};
+
+// dq of one row by itself: a warp, four dims a lane.
+template <class T> __device__ void exact_dq_row(const AttentionArgs &a, const TileUnion &u, uint32_t b, uint32_t kv, uint32_t t, uint32_t q_of_tile, uint32_t head, float delta)
 {
-    constexpr int STAGES = kDqRing<DP, UNIT>, DT = DP / 16;
+    const uint32_t lane = threadIdx.x & 31, d = lane * 4;
+    const bool on = d < a.dim;
+    const T *qr = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)t * a.q_query + (int64_t)head * a.q_head + d;
+    const T *gr = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)t * a.do_query + (int64_t)head * a.do_head + d;
+    float q[4] = {}, g[4] = {}, sum[4] = {};
+    if (on)
+        for (int j = 0; j < 4; ++j) {
+            q[j] = to_f32(qr[j]);
+            g[j] = to_f32(gr[j]);
+        }
+    const float lse = a.lse[((uint64_t)b * a.heads + head) * a.queries + t];
+    for (uint32_t slot = 0; slot < *u.size; ++slot)
+        for (uint64_t seen = u.seen(slot, q_of_tile, a.block); seen; seen &= seen - 1) {
+            const uint32_t key = u.tiles[slot] * kKeyTile + __ffsll((long long)seen) - 1;
+            const T *kr = key_row<T>(a, a.k, a.k_batch, a.k_key, a.k_head, b, kv, key) + d, *vr = key_row<T>(a, a.v, a.v_batch, a.v_key, a.v_head, b, kv, key) + d;
+            float s = 0.f, dp = 0.f;
+            if (on)
+                for (int j = 0; j < 4; ++j) {
+                    s = fmaf(q[j], to_f32(kr[j]), s);
+                    dp = fmaf(g[j], to_f32(vr[j]), dp);
+                }
+#pragma unroll
+            for (int x = 16; x; x >>= 1) {
+                s += __shfl_xor_sync(~0u, s, x);
+                dp += __shfl_xor_sync(~0u, dp, x);
+            }
+            const float ds = exp2f((s * a.scale - lse) * kLog2e) * (dp - delta);
+            if (on)
+                for (int j = 0; j < 4; ++j) sum[j] = fmaf(ds, to_f32(kr[j]), sum[j]);
+        }
+    if (on)
+        for (int j = 0; j < 4; ++j) static_cast<T *>(a.dq)[(((uint64_t)b * a.queries + t) * a.heads + head) * a.dim + d + j] = from_f32<T>(a.scale * sum[j]);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kDqtThreads, 1)
+    block_attention_dq_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap do_map, AttentionArgs a, TcShape shape)
+{
+    using S = DqtSmem<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * kDqUnit<DP, UNIT>), *empty = full + STAGES;
-    volatile uint32_t *gave_up = reinterpret_cast<volatile uint32_t *>(empty + STAGES);
-    BlockUnion u(reinterpret_cast<unsigned char *>(empty + STAGES + 2), tile_queries, a.count, a.num_blocks);
-    const uint32_t t0 = blockIdx.x * tile_queries, b = blockIdx.z;
-    const uint32_t kv = blockIdx.y / chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % chunks * kHeadChunk;
-    const uint32_t heads = min(kHeadChunk, group - head0), queries = min(tile_queries, a.queries - t0);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars), *empty = full + kDqtStages, *rows_full = empty + kDqtStages, *scored = rows_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(landed + 1);  // [0] tensor memory, [1] gave up
+    TileUnion u(smem + S::kLists, shape.queries, a);
+    const uint32_t t0 = blockIdx.x * shape.queries, b = blockIdx.z;
+    const uint32_t kv = blockIdx.y / shape.chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % shape.chunks * shape.heads;
+    const uint32_t heads = min(shape.heads, group - head0), queries = min(shape.queries, a.queries - t0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < kDqtStages; ++s) {
             ptx::mbar_init(&full[s], 1);
-            ptx::mbar_init(&empty[s], kDqWarps);
+            ptx::mbar_init(&empty[s], 1);
         }
-        *gave_up = 0;
+        for (int s = 0; s < 2; ++s) {
+            ptx::mbar_init(&scored[s], 1);
+            ptx::mbar_init(&formed[s], kDqtWarps);
+        }
+        ptx::mbar_init(rows_full, 1);
+        ptx::mbar_init(summed, 1);
+        ptx::mbar_init(landed, 1);
+        misc[1] = 0;
         ptx::fence_mbar_init();
     }
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kDqtCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = misc[0];
     ptx::grid_wait();
     ptx::grid_release();
+    if (warp == kDqtWarps && lane == 0) {
+        ptx::mbar_expect_tx(rows_full, 2 * S::kHalves * shape.queries * shape.heads * 128);
+        for (int h = 0; h < S::kHalves; ++h) {
+            tc::tma_load4(smem + S::kQ + h * 128 * 128, &q_map, h * 64, (int)(kv * group + head0), (int)t0, (int)b, rows_full);
+            tc::tma_load4(smem + S::kDo + h * 128 * 128, &do_map, h * 64, (int)(kv * group + head0), (int)t0, (int)b, rows_full);
+        }
+    }
+    const uint32_t r = threadIdx.x & 127, half = threadIdx.x >> 7, q = r / shape.heads, h = r % shape.heads, head = kv * group + head0 + h;
+    const bool real = half < 2 && q < queries && h < heads;
+    const uint64_t row = ((uint64_t)b * a.queries + t0 + q) * a.heads + head, stat = ((uint64_t)b * a.heads + head) * a.queries + t0 + q;
+    if (half < 2) {  // <dout, out>: two threads take a half of a row each
+        float part = 0.f;
+        if (real) {
+            const T *o = static_cast<const T *>(a.out) + row * a.dim;
+            const T *g = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(t0 + q) * a.do_query + (int64_t)head * a.do_head;
+            for (uint32_t d = half * 8; d < a.dim; d += 16) {
+                const Pack<T, 8> x = load_pack<T, 8>(o + d), y = load_pack<T, 8>(g + d);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) part = fmaf(to_f32(x.x[j]), to_f32(y.x[j]), part);
+            }
+        }
+        reinterpret_cast<float *>(smem + S::kDelta)[half * 128 + r] = part;
+    }
     u.build(a, b, kv, t0, queries);
-    const uint32_t per_block = a.block / UNIT, units = *u.size * per_block;
+    const uint32_t units = *u.size;
 
-    if (warp == kDqWarps) {
-        if (lane == 0) {
-            uint32_t i = 0;
-            for (; i < units && !*gave_up; ++i) {
-                const uint32_t s = i % STAGES;
-                if (!ptx::mbar_wait(&empty[s], ((i / STAGES) & 1u) ^ 1u)) {
-                    *gave_up = 1;
-                    break;
-                }
-                int row, outer;
-                unit_place(a, b, u.blocks[i / per_block], i % per_block * UNIT, row, outer);
-                unsigned char *stage = smem + s * kDqUnit<DP, UNIT>;
-                ptx::mbar_expect_tx(&full[s], kDqUnit<DP, UNIT>);
-#pragma unroll
-                for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + h * UNIT * 128, &k_map, h * 64, (int)kv, row, outer, &full[s]);
-#pragma unroll
-                for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + kDqHalf<DP, UNIT> + h * UNIT * 128, &v_map, h * 64, (int)kv, row, outer, &full[s]);
+    bool ok = true;
+    if (warp == kDqtWarps) {
+        uint32_t phase = 0, i = 0;
+        for (; i < units; ++i) {
+            const uint32_t s = i % kDqtStages;
+            if (!(ok = ptx::mbar_wait_warp(&empty[s], ((i / kDqtStages) & 1u) ^ 1u))) break;
+            if (!(ok = load_key_tile<DP>(smem + S::kRing + s * S::kStage, &k_map, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase))) break;
+        }
+        if (!ok) {
+            misc[1] = 1;
+            if (lane == 0) {  // no copy stays in flight
+                ptx::mbar_wait(rows_full, 0);
+                for (uint32_t j = i > kDqtStages ? i - kDqtStages : 0; j < i; ++j) ptx::mbar_wait(&full[j % kDqtStages], (j / kDqtStages) & 1u);
             }
-            if (*gave_up) {
-                atomicExch(&g_status, 1u);
-                for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j) ptx::mbar_wait(&full[j % STAGES], (j / STAGES) & 1u);
+        } else if (!units && lane == 0)
+            ok = ptx::mbar_wait(rows_full, 0);
+    } else if (warp == kDqtWarps + 1) {
+        if (lane == 0 && units) {
+            constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+            constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_q = tc::idesc(bf16, 128, DP, false, true);
+            const uint32_t base = ptx::smem_u32(smem);
+            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), k_mn = tc::desc_mn(base + S::kRing, 64 * 128);
+            constexpr uint32_t kDoAt = S::kDo >> 4, kValuesAt = (S::kHalves * 64 * 128) >> 4;
+            ok = ptx::mbar_wait(rows_full, 0);
+            uint32_t scores = 0, sums = 0;
+            for (uint32_t idle = 0; ok && sums < units;) {
+                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u)) {
+                    tc::fence_after();
+                    const uint32_t s = sums % kDqtStages, at = s * (S::kStage >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kDqtSum, tmem + kDqtDs + (sums & 1u) * 32 + k * 8, k_mn + (at + k * 128), id_q, sums || k);
+                    tc::commit(&empty[s]);
+                    tc::commit(summed);
+                    ++sums;
+                    idle = 0;
+                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&full[scores % kDqtStages], (scores / kDqtStages) & 1u)) {
+                    tc::fence_after();
+                    const uint32_t at = scores % kDqtStages * (S::kStage >> 4), buffer = tmem + (scores & 1u) * kDqtBuffer;
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d) tc::mma(buffer, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d) tc::mma(buffer + 64, q_k + (kDoAt + (d >> 2) * 1024 + (d & 3) * 2), k_k + (at + kValuesAt + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+                    tc::commit(&scored[scores & 1u]);
+                    ++scores;
+                    idle = 0;
+                } else if (++idle == kTcPolls)
+                    ok = false;
+            }
+            if (!ok) misc[1] = 1;
+        }
+    } else {
+        const float *shares = reinterpret_cast<const float *>(smem + S::kDelta);
+        const float delta = shares[r] + shares[128 + r], lse = real ? a.lse[stat] * kLog2e : 0.f, scale_log2 = a.scale * kLog2e;
+        if (real && half == 0) a.delta[stat] = delta;
+        const uint32_t lanes = tmem + (((warp & 3) * 32) << 16);
+        for (uint32_t i = 0; i < units; ++i) {
+            const uint64_t both = real ? u.seen(i, q, a.block) : 0ull;
+            const uint32_t seen = half ? (uint32_t)(both >> 32) : (uint32_t)both;
+            const uint32_t buffer = lanes + (i & 1u) * kDqtBuffer + half * 32;
+            if (!(ok = ptx::mbar_wait_warp(&scored[i & 1u], (i >> 1) & 1u))) break;
+            tc::fence_after();
+            uint32_t ds[16];
+            if (__any_sync(~0u, seen != 0)) {
+                uint32_t sv[32], dv[32];
+                tc::ld32(buffer, sv);
+                tc::ld32(buffer + 64, dv);
+                tc::wait_ld();
+                // a row that does not name the tile: P is 0 (where D is no number dq is none, and that is formed again)
+                const float minus = seen ? -lse : -INFINITY;
+                const uint64_t scale2 = ptx::pack2(scale_log2, scale_log2), minus2 = ptx::pack2(minus, minus), delta2 = ptx::pack2(-delta, -delta);
+                const bool plain = __all_sync(~0u, seen == 0 || seen == ~0u);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float2 x = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), scale2, minus2));
+                    const uint64_t e = ptx::pack2(tc::exp2_fast(x.x), tc::exp2_fast(x.y)), d = ptx::add2(ptx::pack2(__uint_as_float(dv[2 * c]), __uint_as_float(dv[2 * c + 1])), delta2);
+                    const float2 y = ptx::unpack2(ptx::mul2(e, d));
+                    ds[c] = tc::round2<T>(y.x, y.y);
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) ds[c] &= ((seen >> (2 * c)) & 1u ? 0xffffu : 0u) | ((seen >> (2 * c + 1)) & 1u ? 0xffff0000u : 0u);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) ds[c] = 0;
+            }
+            __syncwarp();
+            tc::st16(lanes + kDqtDs + (i & 1u) * 32 + half * 16, ds);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&formed[i & 1u]);
+        }
+        // the last two, in order: a parity names the one before the last as well as the one to come
+        if (ok && units > 1) ok = ptx::mbar_wait_warp(summed, (units - 2) & 1u);
+        if (ok && units) ok = ptx::mbar_wait_warp(summed, (units - 1) & 1u);
+        tc::fence_after();
+        if (!ok) misc[1] = 1;
+        T *dst = static_cast<T *>(a.dq) + row * a.dim;
+        bool finite = true;
+#pragma unroll 1
+        for (uint32_t c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+            uint32_t o[32];
+            if (units) {
+                tc::ld32(lanes + kDqtSum + c, o);
+                tc::wait_ld();
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t w[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float o0 = units ? __uint_as_float(o[8 * x + 2 * y]) * a.scale : 0.f, o1 = units ? __uint_as_float(o[8 * x + 2 * y + 1]) * a.scale : 0.f;
+                    finite = finite && fabsf(o0) < INFINITY && fabsf(o1) < INFINITY;
+                    w[y] = tc::round2<T>(o0, o1);
+                }
+                if (real && c + 8 * x < a.dim) *reinterpret_cast<uint4 *>(dst + c + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        return;
-    }
-
-    const uint32_t c0 = warp * 8;
-    const uint32_t c = c0 + lane / 4, ct = c / stride, ch = c % stride;
-    const bool row_on = ct < queries && ch < heads;
-    const uint64_t out_row = ((uint64_t)b * a.queries + t0 + ct) * a.heads + kv * group + head0 + ch;
-    uint32_t q[DT][2], g[DT][2];
-    float delta = 0.f;
-    {
-        const T *qr = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)(t0 + ct) * a.q_query + (int64_t)(kv * group + head0 + ch) * a.q_head;
-        const T *gr = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(t0 + ct) * a.do_query + (int64_t)(kv * group + head0 + ch) * a.do_head;
-        const T *orow = static_cast<const T *>(a.out) + out_row * a.dim;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t at = d * 16 + h * 8 + 2 * (lane & 3);
-                const bool on = row_on && at < a.dim;
-                q[d][h] = on ? *reinterpret_cast<const uint32_t *>(qr + at) : 0u;
-                g[d][h] = on ? *reinterpret_cast<const uint32_t *>(gr + at) : 0u;
-                if (on) delta += to_f32(gr[at]) * to_f32(orow[at]) + to_f32(gr[at + 1]) * to_f32(orow[at + 1]);
-            }
-    }
-    delta += __shfl_xor_sync(~0u, delta, 1);
-    delta += __shfl_xor_sync(~0u, delta, 2);
-    const uint64_t stat = ((uint64_t)b * a.heads + kv * group + head0 + ch) * a.queries + t0 + ct;
-    float lse = row_on ? a.lse[stat] : 0.f;
-    if (row_on && (lane & 3) == 0) a.delta[stat] = delta;
-    uint32_t asks = 0;
-    for (uint32_t j = c0 / stride; j <= (c0 + 7) / stride; ++j)
-        if (j < queries && c0 - min(c0, j * stride) < heads) asks |= 1u << j;
-    // the statistics of the two columns this lane holds of a product
-    uint32_t query[2];
-    int sees[2];
-    float base[2], dl[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t from = (2 * (lane & 3) + h) * 4, t = __shfl_sync(~0u, ct, from);
-        const bool on = __shfl_sync(~0u, (int)row_on, from);
-        base[h] = __shfl_sync(~0u, lse, from) * kLog2e;
-        dl[h] = __shfl_sync(~0u, delta, from);
-        query[h] = on ? t : 32u;
-        sees[h] = on ? (int)u.visible[t] : 0;
-    }
-    float dq[DT][4];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.f;
-    const float scale_log2 = a.scale * kLog2e;
-
-    for (uint32_t n = 0; n < units; ++n) {
-        const uint32_t s = n % STAGES, slot = n / per_block, names = u.names[slot];
-        const int first = (int)(u.blocks[slot] * a.block + n % per_block * UNIT);
-        if (!ptx::mbar_wait(&full[s], (n / STAGES) & 1u)) {
-            *gave_up = 1;
-            if (lane == 0) atomicExch(&g_status, 1u);
-            return;
+        for (uint32_t left = __ballot_sync(~0u, real && !finite); left && !misc[1]; left &= left - 1) {
+            const uint32_t from = __ffs(left) - 1, rq = __shfl_sync(~0u, q, from), rh = __shfl_sync(~0u, head, from);
+            const float rd = __shfl_sync(~0u, delta, from);
+            __syncwarp();
+            exact_dq_row<T>(a, u, b, kv, t0 + rq, rq, rh, rd);
         }
-        if (names & asks) {
-            const uint32_t keys = ptx::smem_u32(smem + s * kDqUnit<DP, UNIT>), values = keys + kDqHalf<DP, UNIT>;
-            int limit[2];
-            bool whole = true;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                limit[h] = query[h] < 32u && ((names >> query[h]) & 1u) ? sees[h] - first : 0;
-                whole = whole && (query[h] == 32u || limit[h] >= UNIT);
-            }
-            whole = __all_sync(~0u, whole);
-#pragma unroll
-            for (int k = 0; k < UNIT / 16; ++k) {
-                float sc[4] = {0.f, 0.f, 0.f, 0.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const uint32_t at = (d >> 2) * UNIT * 128 + tc::swizzled(k * 16 + (lane & 15), (d & 3) * 2 + (lane >> 4));
-                    uint32_t f[4];
-                    tc::ldmatrix4(f, keys + at);
-                    tc::mma16<T>(sc, f, q[d][0], q[d][1]);
-                    tc::ldmatrix4(f, values + at);
-                    tc::mma16<T>(dp, f, g[d][0], g[d][1]);
-                }
-                float ds[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int h = j & 1, row = k * 16 + (int)(lane >> 2) + (j >> 1) * 8;
-                    const float p = tc::exp2_fast(fmaf(sc[j], scale_log2, -base[h]));
-                    ds[j] = row < limit[h] ? p * (dp[j] - dl[h]) : 0.f;
-                }
-                const uint32_t b0 = tc::transpose8x8(tc::round2<T>(ds[0], ds[1])), b1 = tc::transpose8x8(tc::round2<T>(ds[2], ds[3]));
-                auto k_frag = [&](uint32_t (&f)[4], int d) {
-                    tc::ldmatrix4_trans(f, keys + (d >> 2) * UNIT * 128 + tc::swizzled(k * 16 + ((lane >> 4) << 3) + (lane & 7), (d & 3) * 2 + ((lane >> 3) & 1)));
-                };
-                if (whole) {
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        uint32_t f[4];
-                        k_frag(f, d);
-                        tc::mma16<T>(dq[d], f, b0, b1);
-                    }
-                } else {  // a pass per query whose part of the unit differs, as in the forward kernel
-                    uint32_t left = names & asks;
-                    bool all = true;
-                    while (left) {
-                        int cut = UNIT;
-                        uint32_t taken = 0;
-                        if (all) {
-                            for (uint32_t m = left; m; m &= m - 1) {
-                                const uint32_t t = __ffs(m) - 1;
-                                if ((int)u.visible[t] - first >= UNIT) taken |= 1u << t;
-                            }
-                            all = false;
-                        } else {
-                            const uint32_t t = __ffs(left) - 1;
-                            taken = 1u << t;
-                            cut = (int)u.visible[t] - first;
-                        }
-                        left &= ~taken;
-                        if (!taken || cut <= k * 16) continue;
-                        const bool mine0 = query[0] < 32u && ((taken >> query[0]) & 1u), mine1 = query[1] < 32u && ((taken >> query[1]) & 1u);
-#pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            float o[4] = {dq[d][0], dq[d][1], dq[d][2], dq[d][3]};
-                            uint32_t f[4];
-                            k_frag(f, d);
-                            if (cut < UNIT) {
-                                const int at = k * 16 + 2 * (int)(lane & 3);
-                                f[0] = keep_keys(f[0], at, cut);
-                                f[1] = keep_keys(f[1], at, cut);
-                                f[2] = keep_keys(f[2], at + 8, cut);
-                                f[3] = keep_keys(f[3], at + 8, cut);
-                            }
-                            tc::mma16<T>(o, f, b0, b1);
-                            if (mine0) {
-                                dq[d][0] = o[0];
-                                dq[d][2] = o[2];
-                            }
-                            if (mine1) {
-                                dq[d][1] = o[1];
-                                dq[d][3] = o[3];
-                            }
-                        }
-                    }
-                }
-            }
-        }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&empty[s]);
     }
-    T *row = static_cast<T *>(a.dq) + out_row * a.dim;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-        const uint32_t lo = tc::transpose8x8(tc::round2<T>(dq[d][0] * a.scale, dq[d][1] * a.scale));
-        const uint32_t hi = tc::transpose8x8(tc::round2<T>(dq[d][2] * a.scale, dq[d][3] * a.scale));
-        const uint32_t at = d * 16 + 2 * (lane & 3);
-        if (row_on && at < a.dim) *reinterpret_cast<uint32_t *>(row + at) = lo;
-        if (row_on && at + 8 < a.dim) *reinterpret_cast<uint32_t *>(row + at + 8) = hi;
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && misc[1]) atomicExch(&g_status, 1u);
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tmem, kDqtCols);
     }
 }
 
 // ---- the pattern turned round ------------------------------------------------------------------------------------------
-constexpr uint32_t kKeyTile = 64;      // keys of a tile of dk and dv
 constexpr uint32_t kItemRows = 4096;   // (query, head) rows that one work item takes at least, unless the tile has fewer
 
 // Where the parts of the workspace begin (bytes), and the sizes they follow from.
@@ -396,7 +430,6 @@ __global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
 constexpr int kDkvWarps = 8, kDkvLoaders = 8;  // warps 0-7 form P and dS, 8-15 load, warp 16 multiplies
 constexpr int kDkvThreads = (kDkvWarps + kDkvLoaders + 1) * 32;
 constexpr int kDkvStages = 2;
-constexpr uint32_t kPolls = 1u << 24;  // of a role that looks at two barriers in turn, before it gives up
 constexpr uint32_t kTmemS = 0, kTmemD = 64, kTmemBuffer = 128, kTmemDv = 256, kTmemDk = 320, kTmemCols = 512;
 
 template <int DP> struct DkvSmem {
@@ -482,7 +515,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const uint32_t n_tiles = (part.y + per_tile - 1) / per_tile;
             announce();
             if (warp == kDkvWarps) {
-                if (k && !(ok = ptx::mbar_wait(summed, (k - 1) & 1u))) break;
+                if (k && !(ok = ptx::mbar_wait_warp(summed, (k - 1) & 1u))) break;
                 if (lane == 0) {
                     ptx::mbar_expect_tx(kv_full, 2 * S::kHalves * 64 * 128);
                     for (int h = 0; h < S::kHalves; ++h) {
@@ -560,7 +593,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                 }
                 announce();  // the tile before has had all of this one's look-up to land
                 const uint32_t s = tile_count % kDkvStages;
-                if (!(ok = ptx::mbar_wait(&empty[s], ((tile_count / kDkvStages) & 1u) ^ 1u))) break;
+                if (!(ok = ptx::mbar_wait_warp(&empty[s], ((tile_count / kDkvStages) & 1u) ^ 1u))) break;
                 if (is_q) reinterpret_cast<uint4 *>(smem + S::kRows)[s * 128 + r] = make_uint4(__float_as_uint(lse), __float_as_uint(delta), (uint32_t)sees, (uint32_t)(sees >> 32));
                 const uint64_t row_at = reinterpret_cast<uint64_t>(row0 + (int64_t)(on ? t : 0u) * row_stride);
                 const uint32_t to = ptx::smem_u32(smem + S::kStage) + (2 * s + (is_q ? 0 : 1)) * S::kTileBytes;
@@ -624,7 +657,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                         tc::commit(&scored[scores & 1u]);
                         ++scores;
                         idle = 0;
-                    } else if (++idle == kPolls) {
+                    } else if (++idle == kTcPolls) {
                         ok = false;
                         break;
                     }
@@ -643,32 +676,37 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const uint32_t n_tiles = tiles_of(it);
             for (uint32_t j = 0; j < n_tiles; ++j, ++tile_count) {
                 const uint32_t s = tile_count % kDkvStages;
-                if (!(ok = ptx::mbar_wait(&full[s], (tile_count / kDkvStages) & 1u))) break;
+                if (!(ok = ptx::mbar_wait_warp(&full[s], (tile_count / kDkvStages) & 1u))) break;
                 const uint4 info = reinterpret_cast<const uint4 *>(smem + S::kRows)[s * 128 + r];
                 const float lse = __uint_as_float(info.x), delta = __uint_as_float(info.y);
                 const uint32_t sees = half ? info.w : info.z;  // a bit per key of this thread's half
                 const uint32_t buffer = lanes + (tile_count & 1u) * kTmemBuffer + half * 32;
-                if (!(ok = ptx::mbar_wait(&scored[tile_count & 1u], (tile_count >> 1) & 1u))) break;
+                if (!(ok = ptx::mbar_wait_warp(&scored[tile_count & 1u], (tile_count >> 1) & 1u))) break;
                 tc::fence_after();
                 uint32_t sv[32], dv[32];
                 tc::ld32(buffer + kTmemS, sv);
                 tc::ld32(buffer + kTmemD, dv);
                 tc::wait_ld();
                 uint32_t pp[16], dd[16];
+                const uint64_t scale2 = ptx::pack2(scale_log2, scale_log2), minus2 = ptx::pack2(-lse, -lse), delta2 = ptx::pack2(-delta, -delta);
+                const bool plain = __all_sync(~0u, sees == ~0u);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
-                    float pv[2], ds[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const bool seen = (sees >> (2 * c + h)) & 1u;
-                        const float e = tc::exp2_fast(fmaf(__uint_as_float(sv[2 * c + h]), scale_log2, -lse));
-                        pv[h] = seen ? e : 0.f;
-                        ds[h] = seen ? e * (__uint_as_float(dv[2 * c + h]) - delta) : 0.f;
-                    }
-                    pp[c] = tc::round2<T>(pv[0], pv[1]);
-                    dd[c] = tc::round2<T>(ds[0], ds[1]);
+                    const float2 x = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), scale2, minus2));
+                    const float2 e = make_float2(tc::exp2_fast(x.x), tc::exp2_fast(x.y));
+                    const float2 y = ptx::unpack2(ptx::mul2(ptx::pack2(e.x, e.y), ptx::add2(ptx::pack2(__uint_as_float(dv[2 * c]), __uint_as_float(dv[2 * c + 1])), delta2)));
+                    pp[c] = tc::round2<T>(e.x, e.y);
+                    dd[c] = tc::round2<T>(y.x, y.y);
                 }
-                if (tile_count && !(ok = ptx::mbar_wait(used, (tile_count - 1) & 1u))) break;
+                if (!plain) {  // keys that a row does not look at: zeros, whatever stands there
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const uint32_t keep = ((sees >> (2 * c)) & 1u ? 0xffffu : 0u) | ((sees >> (2 * c + 1)) & 1u ? 0xffff0000u : 0u);
+                        pp[c] &= keep;
+                        dd[c] &= keep;
+                    }
+                }
+                if (tile_count && !(ok = ptx::mbar_wait_warp(used, (tile_count - 1) & 1u))) break;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const uint32_t at = tc::swizzled(r, half * 4 + c);
@@ -682,7 +720,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             }
             if (!ok) break;
             // ---- the item's sums: warps 0-3 dv, warps 4-7 dk; thread = dim ----
-            if (!(ok = ptx::mbar_wait(summed, k & 1u))) break;
+            if (!(ok = ptx::mbar_wait_warp(summed, k & 1u))) break;
             tc::fence_after();
             const bool is_dk = half != 0;
             const uint32_t d = r, n_items = (p.counts[it.x] + p.item_queries - 1) / p.item_queries;
@@ -747,22 +785,25 @@ template <class T, int DP> __global__ void __launch_bounds__(256) dkv_join_kerne
     }
 }
 
-template <class T, int DP, int UNIT> cudaError_t launch_dq(const AttentionArgs &a, cudaStream_t s)
+template <class T, int DP> cudaError_t launch_dq(const AttentionArgs &a, cudaStream_t s)
 {
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    CUtensorMap k_map{}, v_map{};
+    TcShape shape = tc_shape(a.heads / a.kv_heads, 64);
+    uint32_t bytes = 0;  // fewer queries where their lists are too long
+    for (;; shape.queries /= 2)
+        if ((bytes = DqtSmem<DP>::kLists + TileUnion::bytes(shape.queries, a.count, a.block, a.keys)) <= kSmemMost || shape.queries == 1) break;
+    CUtensorMap k_map{}, v_map{}, q_map, do_map;
+    cudaError_t e = cudaSuccess;
     if (a.keys) {
-        cudaError_t e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, UNIT);
-        if (e == cudaSuccess) e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, UNIT);
-        if (e != cudaSuccess) return e;
+        e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, 64);
+        if (e == cudaSuccess) e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, 64);
     }
-    const uint32_t group = a.heads / a.kv_heads, heads = group < kHeadChunk ? group : kHeadChunk, stride = column_stride(heads), chunks = (group + kHeadChunk - 1) / kHeadChunk;
-    const uint32_t queries = kDqWarps * 8 / stride < kTileQueries ? kDqWarps * 8 / stride : kTileQueries;
-    cudaError_t e = allow_dynamic_smem<block_attention_dq_kernel<T, DP, UNIT>>(160 * 1024);
+    if (e == cudaSuccess) e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, shape.queries, shape.heads);
+    if (e == cudaSuccess) e = tc::make_map(&do_map, bf16, a.dout, a.dim, a.heads, a.queries, a.batch, a.do_head, a.do_query, a.do_batch, shape.queries, shape.heads);
+    if (e == cudaSuccess) e = allow_dynamic_smem<block_attention_dq_kernel<T, DP>>(kSmemMost);
     if (e != cudaSuccess) return e;
-    const uint32_t bytes = kDqRing<DP, UNIT> * (kDqUnit<DP, UNIT> + 16) + 16 + BlockUnion::bytes(queries, a.count, a.num_blocks);
-    const dim3 grid((a.queries + queries - 1) / queries, a.kv_heads * chunks, a.batch);
-    return launch_overlapped(block_attention_dq_kernel<T, DP, UNIT>, grid, dim3((kDqWarps + 1) * 32), bytes, s, k_map, v_map, a, stride, queries, chunks);
+    const dim3 grid((a.queries + shape.queries - 1) / shape.queries, a.kv_heads * shape.chunks, a.batch);
+    return launch_overlapped(block_attention_dq_kernel<T, DP>, grid, dim3(kDqtThreads), bytes, s, k_map, v_map, q_map, do_map, a, shape);
 }
 
 template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count, cudaStream_t s)
@@ -771,7 +812,7 @@ template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count
     const GradLayout l(a);
     char *w = static_cast<char *>(a.workspace);
     a.delta = reinterpret_cast<float *>(w + l.delta);
-    cudaError_t e = a.block == 16 ? launch_dq<T, DP, 16>(a, s) : a.block == 32 ? launch_dq<T, DP, 32>(a, s) : launch_dq<T, DP, 64>(a, s);
+    cudaError_t e = launch_dq<T, DP>(a, s);
     if (e != cudaSuccess || !a.keys) return e;
     TurnArgs p{};
     p.a = a;

@@ -121,7 +121,7 @@ template <class T> __global__ void __launch_bounds__(kScoreThreads) block_scores
     } else if (warp < 4) {
         // accumulator -> rows of scores, 32 x 32 at a time through shared memory (the ring is free by then), so that a store is 128
         // contiguous bytes of one row whatever the row's alignment
-        if (ptx::mbar_wait(done, 0)) {
+        if (ptx::mbar_wait_warp(done, 0)) {
             tc::fence_after();
             float *tile = reinterpret_cast<float *>(smem) + warp * 32 * 33;
             float *out = a.scores + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0 + warp * 32) * a.blocks + n0;

@@ -374,15 +374,25 @@ def test_rows_that_see_nothing_and_keys_that_nobody_sees(dtype, form):
     got = check_attention(q, k, v, blocks, block, visible)
     assert not got[0][visible <= 0].any() and not got[1][visible <= 0].any()
     assert not got[0][0, 5].any()
-    # a key that later queries see may hold anything as far as earlier ones are concerned
+    # a key that later queries see may hold anything as far as earlier ones are concerned, and so may a block that others name
     late = default_visible(batch, queries, keys)
     q, k, v = attention_inputs(dtype, batch, queries, keys, kv, group, dim)
-    clean = ops.block_attention(q, k, v, blocks, block, late)
+    blocks[:, :, : queries // 2] = torch.where(blocks[:, :, : queries // 2] == 0, -1, blocks[:, :, : queries // 2])
+    pattern = pattern_of(blocks, block, keys, late)
+    clean = ~pattern[..., [0, -1]].any(-1).any(1)  # queries that look at neither key 0 nor the last
+    dout = torch.randn(q.shape, device="cuda").to(dtype)
+    (want, bound), (want_dq, bound_dq) = attention_reference(q, k, v, pattern, 1 / math.sqrt(dim), dout)[:2]
     k[:, -1], v[:, -1] = math.nan, math.inf
-    assert torch.equal(ops.block_attention(q, k, v, blocks, block, late)[:, :-1], clean[:, :-1])
-    few = slice(queries - 3, queries)
-    clean_few = ops.block_attention(q[:, few], k.nan_to_num(), v.nan_to_num(posinf=0.0), blocks[:, :, few].contiguous(), block, late[:, few].contiguous())
-    assert torch.equal(ops.block_attention(q[:, few], k, v, blocks[:, :, few].contiguous(), block, late[:, few].contiguous())[:, :-1], clean_few[:, :-1])
+    k[:, 0], v[:, 0] = -math.inf, math.nan
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = ops.block_attention(*leaves, blocks, block, late)
+    within(out[clean], want[clean], bound[clean])
+    (dq,) = torch.autograd.grad(out, q, dout)
+    within(dq[clean], want_dq[clean], bound_dq[clean])
+    few = slice(queries - 4, queries)
+    with torch.no_grad():
+        out = ops.block_attention(q[:, few], k, v, blocks[:, :, few].contiguous(), block, late[:, few].contiguous())
+    within(out[clean[:, few]], want[:, few][clean[:, few]], bound[:, few][clean[:, few]])
 
 
 @pytest.mark.gpu
