@@ -143,9 +143,9 @@ template <int DP> struct TcSmem {
     static constexpr int kHalves = DP / 64;
     static constexpr int kQ = 0;
     static constexpr int kRing = kHalves * 128 * 128;
-    static constexpr int kStage = 2 * kHalves * 64 * 128;
-    static constexpr int kBars = kRing + kTcStages * kStage;
-    static constexpr int kLists = kBars + 128;
+    static constexpr int kTile = kHalves * 64 * 128;      // keys of a stage, or its values
+    static constexpr int kBars = kRing + 2 * kTcStages * kTile;  // stages of keys, then of values
+    static constexpr int kLists = kBars + 144;
 };
 
 // One row by itself: a warp, four dims a lane, over the keys its query looks at.
@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
     using S = TcSmem<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars), *empty = full + kTcStages, *q_full = empty + kTcStages, *scored = q_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
+    // keys are given back when S is complete, values when O is: a tile's keys are on their way while the one before is summed
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + S::kBars), *k_empty = k_full + kTcStages, *v_full = k_empty + kTcStages, *v_empty = v_full + kTcStages, *q_full = v_empty + kTcStages, *scored = q_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(landed + 1);  // [0] tensor memory, [1] gave up
     TileUnion u(smem + S::kLists, shape.queries, a);
     const uint32_t t0 = blockIdx.x * shape.queries, b = blockIdx.z;
@@ -192,8 +193,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
     const uint32_t heads = min(shape.heads, group - head0), queries = min(shape.queries, a.queries - t0);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kTcStages; ++s) {
-            ptx::mbar_init(&full[s], 1);
-            ptx::mbar_init(&empty[s], 1);
+            ptx::mbar_init(&k_full[s], 1);
+            ptx::mbar_init(&k_empty[s], 1);
+            ptx::mbar_init(&v_full[s], 1);
+            ptx::mbar_init(&v_empty[s], 1);
             ptx::mbar_init(&scored[s], 1);
             ptx::mbar_init(&formed[s], 4);  // per buffer: a warp without work may be a tile ahead of the others
         }
@@ -222,14 +225,19 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
         uint32_t phase = 0, i = 0;
         for (; i < units; ++i) {
             const uint32_t s = i % kTcStages;
-            if (!(ok = ptx::mbar_wait_warp(&empty[s], ((i / kTcStages) & 1u) ^ 1u))) break;
-            if (!(ok = load_key_tile<DP>(smem + S::kRing + s * S::kStage, &k_map, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase))) break;
+            const uint32_t parity = ((i / kTcStages) & 1u) ^ 1u;
+            unsigned char *keys = smem + S::kRing + s * S::kTile;
+            if (!(ok = ptx::mbar_wait_warp(&k_empty[s], parity) && load_key_tile<DP>(keys, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &k_full[s], landed, phase))) break;
+            if (!(ok = ptx::mbar_wait_warp(&v_empty[s], parity) && load_key_tile<DP>(keys + kTcStages * S::kTile, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &v_full[s], landed, phase))) break;
         }
         if (!ok) {
             misc[1] = 1;
             if (lane == 0) {  // no copy stays in flight
                 ptx::mbar_wait(q_full, 0);
-                for (uint32_t j = i > kTcStages ? i - kTcStages : 0; j < i; ++j) ptx::mbar_wait(&full[j % kTcStages], (j / kTcStages) & 1u);
+                for (uint32_t j = i > kTcStages ? i - kTcStages : 0; j <= i && j < units; ++j) {  // of tile i perhaps the keys alone: that wait runs out
+                    ptx::mbar_wait(&k_full[j % kTcStages], (j / kTcStages) & 1u);
+                    if (j < i) ptx::mbar_wait(&v_full[j % kTcStages], (j / kTcStages) & 1u);
+                }
             }
         } else if (!units && lane == 0)
             ok = ptx::mbar_wait(q_full, 0);
@@ -238,24 +246,25 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
             constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
             constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_o = tc::idesc(bf16, 128, DP, false, true);
             const uint32_t base = ptx::smem_u32(smem);
-            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), v_mn = tc::desc_mn(base + S::kRing + S::kHalves * 64 * 128, 64 * 128);
+            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), v_mn = tc::desc_mn(base + S::kRing + kTcStages * S::kTile, 64 * 128);
             ok = ptx::mbar_wait(q_full, 0);
             uint32_t scores = 0, sums = 0;
             for (uint32_t idle = 0; ok && sums < units;) {
-                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u)) {
+                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u) && ptx::mbar_test(&v_full[sums % kTcStages], (sums / kTcStages) & 1u)) {
                     tc::fence_after();
-                    const uint32_t s = sums % kTcStages, at = s * (S::kStage >> 4);
+                    const uint32_t s = sums % kTcStages, at = s * (S::kTile >> 4);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kTcO, tmem + (sums & 1u) * 64 + k * 8, v_mn + (at + k * 128), id_o, sums || k);
-                    tc::commit(&empty[s]);
+                    tc::commit(&v_empty[s]);
                     tc::commit(summed);
                     ++sums;
                     idle = 0;
-                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&full[scores % kTcStages], (scores / kTcStages) & 1u)) {
+                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&k_full[scores % kTcStages], (scores / kTcStages) & 1u)) {
                     tc::fence_after();
-                    const uint32_t at = scores % kTcStages * (S::kStage >> 4);
+                    const uint32_t at = scores % kTcStages * (S::kTile >> 4);
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) tc::mma(tmem + (scores & 1u) * 64, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
+                    tc::commit(&k_empty[scores % kTcStages]);
                     tc::commit(&scored[scores & 1u]);
                     ++scores;
                     idle = 0;

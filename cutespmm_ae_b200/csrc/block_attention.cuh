@@ -156,19 +156,18 @@ inline TcShape tc_shape(uint32_t group, uint32_t box_rows)
 constexpr uint32_t kSmemMost = 227 * 1024;
 constexpr uint32_t kTcPolls = 1u << 24;  // of a role that looks at two barriers in turn, before it gives up
 
-// One warp brings the keys and values of a tile into shared memory: per operand DP / 64 tiles of 64 rows x 128 bytes, swizzled.  Rows
-// that none of the queries sees become zeros: whatever a cache holds behind the last key, 0 times it has to be 0.  box_rows: rows of a
-// box of the maps (64, or the size of a page).  Returns false when a wait gave up.
+// One warp brings the keys (or values) of a tile into shared memory: DP / 64 tiles of 64 rows x 128 bytes, swizzled.  Rows that none of the
+// queries sees become zeros: whatever a cache holds behind the last key, 0 times it has to be 0.  box_rows: rows of a box of the map (64,
+// or the size of a page).  Returns false when a wait gave up.
 template <int DP>
-__device__ __forceinline__ bool load_key_tile(unsigned char *stage, const CUtensorMap *k_map, const CUtensorMap *v_map, const AttentionArgs &a, uint32_t b, uint32_t kv, uint32_t tile,
-                                              uint32_t visible, uint32_t box_rows, uint64_t *full, uint64_t *landed, uint32_t &landed_phase)
+__device__ __forceinline__ bool load_key_tile(unsigned char *to, const CUtensorMap *map, const AttentionArgs &a, uint32_t b, uint32_t kv, uint32_t tile, uint32_t visible, uint32_t box_rows,
+                                              uint64_t *full, uint64_t *landed, uint32_t &landed_phase)
 {
-    constexpr uint32_t kOperand = DP / 64 * kKeyTile * 128;
     const uint32_t lane = threadIdx.x & 31, first = tile * kKeyTile;
     const bool cut = first + kKeyTile > visible;
     uint64_t *bar = cut ? landed : full;
     if (lane == 0) {
-        ptx::mbar_expect_tx(bar, 2 * kOperand);
+        ptx::mbar_expect_tx(bar, DP / 64 * kKeyTile * 128);
         for (uint32_t r = 0; r < kKeyTile; r += box_rows) {
             int row = (int)(first + r), outer = (int)b;
             if (a.pages) {
@@ -177,21 +176,16 @@ __device__ __forceinline__ bool load_key_tile(unsigned char *stage, const CUtens
                 outer = j < a.page_cols ? a.pages[(uint64_t)b * a.page_cols + j] : -1;  // what is no page arrives as zeros
             }
 #pragma unroll
-            for (int h = 0; h < DP / 64; ++h) {
-                tc::tma_load4(stage + h * kKeyTile * 128 + r * 128, k_map, h * 64, (int)kv, row, outer, bar);
-                tc::tma_load4(stage + kOperand + h * kKeyTile * 128 + r * 128, v_map, h * 64, (int)kv, row, outer, bar);
-            }
+            for (int h = 0; h < DP / 64; ++h) tc::tma_load4(to + h * kKeyTile * 128 + r * 128, map, h * 64, (int)kv, row, outer, bar);
         }
     }
     __syncwarp();
     if (!cut) return true;
     const bool ok = ptx::mbar_wait_warp(landed, landed_phase);
     landed_phase ^= 1u;
-    const uint32_t from = visible > first ? visible - first : 0u;
-    for (uint32_t i = lane; i < 2 * (DP / 64) * (kKeyTile - from) * 8; i += 32) {
-        const uint32_t operand = i / ((kKeyTile - from) * 8), row = from + i % ((kKeyTile - from) * 8) / 8;
-        *reinterpret_cast<uint4 *>(stage + operand * kKeyTile * 128 + row * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
-    }
+    constexpr uint32_t kPieces = DP / 8;  // 16-byte pieces of a row
+    unsigned char *at = to + lane % kPieces / 8 * kKeyTile * 128 + lane % 8 * 16;
+    for (uint32_t row = (visible > first ? visible - first : 0u) + lane / kPieces; row < kKeyTile; row += 32 / kPieces) *reinterpret_cast<uint4 *>(at + row * 128) = make_uint4(0, 0, 0, 0);
     ptx::fence_async_smem();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(full);

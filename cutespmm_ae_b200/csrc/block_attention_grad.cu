@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kDqtThreads, 1)
     const uint32_t heads = min(shape.heads, group - head0), queries = min(shape.queries, a.queries - t0);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kDqtStages; ++s) {
-            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&full[s], 2);  // keys and values
             ptx::mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -145,7 +145,10 @@ __global__ void __launch_bounds__(kDqtThreads, 1)
         for (; i < units; ++i) {
             const uint32_t s = i % kDqtStages;
             if (!(ok = ptx::mbar_wait_warp(&empty[s], ((i / kDqtStages) & 1u) ^ 1u))) break;
-            if (!(ok = load_key_tile<DP>(smem + S::kRing + s * S::kStage, &k_map, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase))) break;
+            unsigned char *keys = smem + S::kRing + s * S::kStage;
+            if (!(ok = load_key_tile<DP>(keys, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase) &&
+                       load_key_tile<DP>(keys + S::kStage / 2, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase)))
+                break;
         }
         if (!ok) {
             misc[1] = 1;
