@@ -126,7 +126,8 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 // ---- a tile of queries -------------------------------------------------------------------------------------------------
 // 128 rows -- up to 32 neighbouring queries with all heads of a group (or a chunk of them) -- against the union of the tiles of 64 keys that they name:
 //     S = Q K^T (128 x 64, two buffers in tensor memory);  P from registers back into S's columns as 16-bit operand;  O += P V.
-// Warps 0-3 hold a row each lane (a row's maximum and sum need no other lane), warp 4 loads, warp 5 multiplies whatever is ready.
+// Warps 0-3 hold a row each lane (a row's maximum and sum need no other lane), warp 4 loads, warp 5 issues S, warp 6 O: one warp for both
+// spent a third of a tile's time between them.
 // Rows whose query does not name a tile have P = 0 there.  Multiplying only what is named, on mma.sync with a query's eight heads as the columns of
 // an instruction, was slower for every group, block size and dim tried with the blocks of a selection: 8192 queries, 32 heads, 16 blocks of 64, where
 // 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 510; 4096 queries, one head to a group, 16 blocks of 16 302 against 226.
@@ -134,8 +135,8 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 // tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM: one multiplies while the other's rows are at work.
 // 0 times a value that is no number is not 0: rows of V behind the last visible key are zeroed as they land, and a row whose result is
 // not finite is formed again, key by key, from what its query looks at (exact_row).
-constexpr int kTcThreads = 192;
-constexpr int kTcStages = 2;
+constexpr int kTcThreads = 224;
+constexpr int kTcStages = 2;  // of keys, of values, and of S in tensor memory
 constexpr uint32_t kTcO = 128, kTcCols = 256;  // columns of tensor memory: two buffers of S, O
 constexpr float kRaise = 8.f;                  // log2
 
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // keys are given back when S is complete, values when O is: a tile's keys are on their way while the one before is summed
-    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + S::kBars), *k_empty = k_full + kTcStages, *v_full = k_empty + kTcStages, *v_empty = v_full + kTcStages, *q_full = v_empty + kTcStages, *scored = q_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + S::kBars), *v_full = k_full + kTcStages, *scored = v_full + kTcStages, *formed = scored + kTcStages, *summed = formed + kTcStages, *q_full = summed + kTcStages, *landed = q_full + 1;
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(landed + 1);  // [0] tensor memory, [1] gave up
     TileUnion u(smem + S::kLists, shape.queries, a);
     const uint32_t t0 = blockIdx.x * shape.queries, b = blockIdx.z;
@@ -194,14 +195,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
     if (threadIdx.x == 0) {
         for (int s = 0; s < kTcStages; ++s) {
             ptx::mbar_init(&k_full[s], 1);
-            ptx::mbar_init(&k_empty[s], 1);
             ptx::mbar_init(&v_full[s], 1);
-            ptx::mbar_init(&v_empty[s], 1);
             ptx::mbar_init(&scored[s], 1);
             ptx::mbar_init(&formed[s], 4);  // per buffer: a warp without work may be a tile ahead of the others
+            ptx::mbar_init(&summed[s], 1);
         }
         ptx::mbar_init(q_full, 1);
-        ptx::mbar_init(summed, 1);
         ptx::mbar_init(landed, 1);
         misc[1] = 0;
         ptx::fence_mbar_init();
@@ -227,8 +226,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
             const uint32_t s = i % kTcStages;
             const uint32_t parity = ((i / kTcStages) & 1u) ^ 1u;
             unsigned char *keys = smem + S::kRing + s * S::kTile;
-            if (!(ok = ptx::mbar_wait_warp(&k_empty[s], parity) && load_key_tile<DP>(keys, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &k_full[s], landed, phase))) break;
-            if (!(ok = ptx::mbar_wait_warp(&v_empty[s], parity) && load_key_tile<DP>(keys + kTcStages * S::kTile, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &v_full[s], landed, phase))) break;
+            if (!(ok = ptx::mbar_wait_warp(&scored[s], parity) && load_key_tile<DP>(keys, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &k_full[s], landed, phase))) break;
+            if (!(ok = ptx::mbar_wait_warp(&summed[s], parity) && load_key_tile<DP>(keys + kTcStages * S::kTile, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &v_full[s], landed, phase))) break;
         }
         if (!ok) {
             misc[1] = 1;
@@ -243,33 +242,33 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
             ok = ptx::mbar_wait(q_full, 0);
     } else if (warp == 5) {
         if (lane == 0 && units) {
-            constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-            constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_o = tc::idesc(bf16, 128, DP, false, true);
+            constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, 128, 64);
             const uint32_t base = ptx::smem_u32(smem);
-            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), v_mn = tc::desc_mn(base + S::kRing + kTcStages * S::kTile, 64 * 128);
+            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing);
             ok = ptx::mbar_wait(q_full, 0);
-            uint32_t scores = 0, sums = 0;
-            for (uint32_t idle = 0; ok && sums < units;) {
-                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u) && ptx::mbar_test(&v_full[sums % kTcStages], (sums / kTcStages) & 1u)) {
-                    tc::fence_after();
-                    const uint32_t s = sums % kTcStages, at = s * (S::kTile >> 4);
+            for (uint32_t i = 0; ok && i < units; ++i) {
+                const uint32_t s = i % kTcStages, parity = (i / kTcStages) & 1u;
+                // the buffer held P two tiles ago
+                if (!(ok = ptx::mbar_wait(&k_full[s], parity) && ptx::mbar_wait(&summed[s], parity ^ 1u))) break;
+                tc::fence_after();
+                const uint32_t at = s * (S::kTile >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kTcO, tmem + (sums & 1u) * 64 + k * 8, v_mn + (at + k * 128), id_o, sums || k);
-                    tc::commit(&v_empty[s]);
-                    tc::commit(summed);
-                    ++sums;
-                    idle = 0;
-                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&k_full[scores % kTcStages], (scores / kTcStages) & 1u)) {
-                    tc::fence_after();
-                    const uint32_t at = scores % kTcStages * (S::kTile >> 4);
+                for (int d = 0; d < DP / 16; ++d) tc::mma(tmem + s * 64, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id, d != 0);
+                tc::commit(&scored[s]);
+            }
+            if (!ok) misc[1] = 1;
+        }
+    } else if (warp == 6) {
+        if (lane == 0) {
+            constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, 128, DP, false, true);
+            const uint64_t v_mn = tc::desc_mn(ptx::smem_u32(smem) + S::kRing + kTcStages * S::kTile, 64 * 128);
+            for (uint32_t i = 0; i < units; ++i) {
+                const uint32_t s = i % kTcStages, parity = (i / kTcStages) & 1u, at = s * (S::kTile >> 4);
+                if (!(ok = ptx::mbar_wait(&v_full[s], parity) && ptx::mbar_wait(&formed[s], parity))) break;
+                tc::fence_after();
 #pragma unroll
-                    for (int d = 0; d < DP / 16; ++d) tc::mma(tmem + (scores & 1u) * 64, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
-                    tc::commit(&k_empty[scores % kTcStages]);
-                    tc::commit(&scored[scores & 1u]);
-                    ++scores;
-                    idle = 0;
-                } else if (++idle == kTcPolls)
-                    ok = false;
+                for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kTcO, tmem + s * 64 + k * 8, v_mn + (at + k * 128), id, i || k);
+                tc::commit(&summed[s]);
             }
             if (!ok) misc[1] = 1;
         }
@@ -315,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
                     }
                 }
                 if (__any_sync(~0u, raise)) {
-                    if (!(ok = ptx::mbar_wait_warp(summed, (i - 1) & 1u))) break;  // the products in flight add to O
+                    if (!(ok = ptx::mbar_wait_warp(&summed[(i - 1) & 1u], ((i - 1) >> 1) & 1u))) break;  // the products in flight add to O
                     tc::fence_after();
 #pragma unroll 1
                     for (uint32_t c = 0; c < DP; c += 32) {
@@ -351,9 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&formed[i & 1u]);
         }
-        // the last two, in order: a parity names the one before the last as well as the one to come
-        if (ok && units > 1) ok = ptx::mbar_wait_warp(summed, (units - 2) & 1u);
-        if (ok && units) ok = ptx::mbar_wait_warp(summed, (units - 1) & 1u);
+        if (ok && units) ok = ptx::mbar_wait_warp(&summed[(units - 1) & 1u], ((units - 1) >> 1) & 1u);
         tc::fence_after();
         if (!ok) misc[1] = 1;
         const float inv = sum > 0.f ? 1.f / sum : 0.f;

@@ -82,20 +82,20 @@ struct TileUnion {
     {
         const uint32_t w = words(a.keys), n = queries * a.count, per = tiles_of_block(a.block);
         const int32_t *src = a.blocks + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0) * a.count;
+        const uint32_t most_names = slots(queries, a.count, a.block, a.keys) * parts;
         for (uint32_t i = threadIdx.x; i < w; i += blockDim.x) bits[i] = 0;
+        for (uint32_t i = threadIdx.x; i < most_names; i += blockDim.x) names[i] = 0;
         for (uint32_t i = threadIdx.x; i < queries; i += blockDim.x) visible[i] = visible_keys(a, b, t0 + i);
-        __syncthreads();
-        auto each = [&](auto &&fn) {  // fn(tile, part, query) for what every query names and sees a part of
-            for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-                const uint32_t q = i / a.count;
-                const int32_t j = src[i];
-                if (!block_counts(a, b, j, visible[q])) continue;
-                const uint64_t first = (uint64_t)j * a.block;
-                for (uint32_t x = 0; x < per; ++x)
-                    if (first + x * kKeyTile < visible[q]) fn((uint32_t)(first / kKeyTile) + x, (uint32_t)(first % kKeyTile) / a.block, q);
-            }
+        auto each = [&](uint32_t i, int32_t j, uint32_t see, auto &&fn) {  // fn(tile, part, query) for what entry i names and its query sees a part of
+            if (!block_counts(a, b, j, see)) return;
+            const uint64_t first = (uint64_t)j * a.block;
+            for (uint32_t x = 0; x < per; ++x)
+                if (first + x * kKeyTile < see) fn((uint32_t)(first / kKeyTile) + x, (uint32_t)(first % kKeyTile) / a.block, i / a.count);
         };
-        each([&](uint32_t tile, uint32_t, uint32_t) { atomicOr(&bits[tile >> 5], 1u << (tile & 31)); });
+        const int32_t mine = threadIdx.x < n ? src[threadIdx.x] : -1;  // on its way during the barrier
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+            each(i, i == threadIdx.x ? mine : src[i], visible[i / a.count], [&](uint32_t tile, uint32_t, uint32_t) { atomicOr(&bits[tile >> 5], 1u << (tile & 31)); });
         __syncthreads();
         if (threadIdx.x < 32) {
             uint32_t sum = 0, most = 0;
@@ -118,13 +118,12 @@ struct TileUnion {
             }
         }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < size[0] * parts; i += blockDim.x) names[i] = 0;
-        __syncthreads();
-        each([&](uint32_t tile, uint32_t part, uint32_t q) {
-            const uint32_t at = before[tile >> 5] + __popc(bits[tile >> 5] & ((1u << (tile & 31)) - 1u));
-            tiles[at] = tile;
-            atomicOr(&names[at * parts + part], 1u << q);
-        });
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+            each(i, i == threadIdx.x ? mine : src[i], visible[i / a.count], [&](uint32_t tile, uint32_t part, uint32_t q) {
+                const uint32_t at = before[tile >> 5] + __popc(bits[tile >> 5] & ((1u << (tile & 31)) - 1u));
+                tiles[at] = tile;
+                atomicOr(&names[at * parts + part], 1u << q);
+            });
         __syncthreads();
     }
     // the keys of a tile that query q looks at, a bit each

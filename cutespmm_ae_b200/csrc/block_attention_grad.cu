@@ -26,19 +26,19 @@ __device__ uint32_t g_status;  // set to 1 (dq) or 2 (dk, dv) when a bounded wai
 
 // ---- dq ----------------------------------------------------------------------------------------------------------------
 // The forward kernel's 128 rows and union of key tiles.  Per tile S = Q K^T and D = dO V^T (128 x 64, two buffers of tensor memory), dS from
-// registers into tensor memory as 16-bit operand, dQ += dS K with the same bytes of K.  Eight warps form dS: a row's lse and delta are one
-// value each for the whole kernel, two threads share a row.  A row whose dq is not finite is formed again from what its query looks at.
-constexpr int kDqtWarps = 8, kDqtThreads = (kDqtWarps + 2) * 32, kDqtStages = 3;
-constexpr uint32_t kDqtBuffer = 128, kDqtSum = 256, kDqtDs = 384, kDqtCols = 512;
+// registers back into S's columns as 16-bit operand, dQ += dS K with the same bytes of K.  Q and dO stay in tensor memory for the whole kernel: an
+// operand A in shared memory would be read again for every 16 dims, 6 KB for 32 cycles of multiplying.  Eight warps form dS: a row's lse and
+// delta are one value each, two threads share a row.  Warp 8 loads, warp 9 issues S and D, warp 10 dQ.  A row whose dq is not finite is formed again from
+// what its query looks at.
+constexpr int kDqWarps = 8, kDqThreads = (kDqWarps + 3) * 32, kDqStages = 4;
+constexpr uint32_t kDqBuffer = 128, kDqSum = 256, kDqQ = 384, kDqDo = 448, kDqCols = 512;
 
-template <int DP> struct DqtSmem {
-    static constexpr int kHalves = DP / 64;
-    static constexpr int kQ = 0, kDo = kHalves * 128 * 128;
-    static constexpr int kRing = 2 * kHalves * 128 * 128;
-    static constexpr int kStage = 2 * kHalves * 64 * 128;
-    static constexpr int kDelta = kRing + kDqtStages * kStage;  // two shares of delta per row
+template <int DP> struct DqSmem {
+    static constexpr int kTile = DP / 64 * 64 * 128;
+    static constexpr int kKeys = 0, kValues = kDqStages * kTile;
+    static constexpr int kDelta = 2 * kDqStages * kTile;  // two shares of delta per row
     static constexpr int kBars = kDelta + 2 * 128 * 4;
-    static constexpr int kLists = kBars + 128;
+    static constexpr int kLists = kBars + 192;
 };
 
 // dq of one row by itself: a warp, four dims a lane.
@@ -78,130 +78,144 @@ template <class T> __device__ void exact_dq_row(const AttentionArgs &a, const Ti
         for (int j = 0; j < 4; ++j) static_cast<T *>(a.dq)[(((uint64_t)b * a.queries + t) * a.heads + head) * a.dim + d + j] = from_f32<T>(a.scale * sum[j]);
 }
 
-template <class T, int DP>
-__global__ void __launch_bounds__(kDqtThreads, 1)
-    block_attention_dq_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap do_map, AttentionArgs a, TcShape shape)
+// 8 V columns of tensor memory from V 16-byte pieces of a row
+template <class T, int V> __device__ __forceinline__ void row_to_tmem(uint32_t taddr, const T *src, uint32_t dims)
 {
-    using S = DqtSmem<DP>;
+    uint32_t w[4 * V];
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+        const uint4 u = 8 * x < (int)dims ? __ldg(reinterpret_cast<const uint4 *>(src) + x) : make_uint4(0, 0, 0, 0);
+        w[4 * x] = u.x;
+        w[4 * x + 1] = u.y;
+        w[4 * x + 2] = u.z;
+        w[4 * x + 3] = u.w;
+    }
+    if constexpr (V == 8) tc::st32(taddr, w);
+    else tc::st16(taddr, w);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kDqThreads, 1) block_attention_dq_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, AttentionArgs a, TcShape shape)
+{
+    using S = DqSmem<DP>;
+    constexpr uint32_t kHalfDims = DP / 2;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars), *empty = full + kDqtStages, *rows_full = empty + kDqtStages, *scored = rows_full + 1, *formed = scored + 2, *summed = formed + 2, *landed = summed + 1;
+    // a stage's values are given back when S and D are complete (scored), its keys when dQ is (summed)
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + S::kBars), *v_full = k_full + kDqStages, *scored = v_full + kDqStages, *formed = scored + kDqStages, *summed = formed + kDqStages, *rows_in = summed + kDqStages, *landed = rows_in + 1;
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(landed + 1);  // [0] tensor memory, [1] gave up
     TileUnion u(smem + S::kLists, shape.queries, a);
     const uint32_t t0 = blockIdx.x * shape.queries, b = blockIdx.z;
     const uint32_t kv = blockIdx.y / shape.chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % shape.chunks * shape.heads;
     const uint32_t heads = min(shape.heads, group - head0), queries = min(shape.queries, a.queries - t0);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kDqtStages; ++s) {
-            ptx::mbar_init(&full[s], 2);  // keys and values
-            ptx::mbar_init(&empty[s], 1);
-        }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < kDqStages; ++s) {
+            ptx::mbar_init(&k_full[s], 1);
+            ptx::mbar_init(&v_full[s], 1);
             ptx::mbar_init(&scored[s], 1);
-            ptx::mbar_init(&formed[s], kDqtWarps);
+            ptx::mbar_init(&formed[s], kDqWarps);
+            ptx::mbar_init(&summed[s], 1);
         }
-        ptx::mbar_init(rows_full, 1);
-        ptx::mbar_init(summed, 1);
+        ptx::mbar_init(rows_in, kDqWarps);
         ptx::mbar_init(landed, 1);
         misc[1] = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kDqtCols);
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kDqCols);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = misc[0];
     ptx::grid_wait();
     ptx::grid_release();
-    if (warp == kDqtWarps && lane == 0) {
-        ptx::mbar_expect_tx(rows_full, 2 * S::kHalves * shape.queries * shape.heads * 128);
-        for (int h = 0; h < S::kHalves; ++h) {
-            tc::tma_load4(smem + S::kQ + h * 128 * 128, &q_map, h * 64, (int)(kv * group + head0), (int)t0, (int)b, rows_full);
-            tc::tma_load4(smem + S::kDo + h * 128 * 128, &do_map, h * 64, (int)(kv * group + head0), (int)t0, (int)b, rows_full);
-        }
-    }
-    const uint32_t r = threadIdx.x & 127, half = threadIdx.x >> 7, q = r / shape.heads, h = r % shape.heads, head = kv * group + head0 + h;
-    const bool real = half < 2 && q < queries && h < heads;
-    const uint64_t row = ((uint64_t)b * a.queries + t0 + q) * a.heads + head, stat = ((uint64_t)b * a.heads + head) * a.queries + t0 + q;
-    if (half < 2) {  // <dout, out>: two threads take a half of a row each
-        float part = 0.f;
-        if (real) {
-            const T *o = static_cast<const T *>(a.out) + row * a.dim;
-            const T *g = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)(t0 + q) * a.do_query + (int64_t)head * a.do_head;
-            for (uint32_t d = half * 8; d < a.dim; d += 16) {
-                const Pack<T, 8> x = load_pack<T, 8>(o + d), y = load_pack<T, 8>(g + d);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) part = fmaf(to_f32(x.x[j]), to_f32(y.x[j]), part);
-            }
-        }
-        reinterpret_cast<float *>(smem + S::kDelta)[half * 128 + r] = part;
-    }
     u.build(a, b, kv, t0, queries);
     const uint32_t units = *u.size;
 
     bool ok = true;
-    if (warp == kDqtWarps) {
+    if (warp == kDqWarps) {
         uint32_t phase = 0, i = 0;
         for (; i < units; ++i) {
-            const uint32_t s = i % kDqtStages;
-            if (!(ok = ptx::mbar_wait_warp(&empty[s], ((i / kDqtStages) & 1u) ^ 1u))) break;
-            unsigned char *keys = smem + S::kRing + s * S::kStage;
-            if (!(ok = load_key_tile<DP>(keys, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase) &&
-                       load_key_tile<DP>(keys + S::kStage / 2, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &full[s], landed, phase)))
-                break;
+            const uint32_t s = i % kDqStages, parity = ((i / kDqStages) & 1u) ^ 1u;
+            ok = ptx::mbar_wait_warp(&summed[s], parity) &&
+                 load_key_tile<DP>(smem + S::kKeys + s * S::kTile, &k_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &k_full[s], landed, phase) &&
+                 load_key_tile<DP>(smem + S::kValues + s * S::kTile, &v_map, a, b, kv, u.tiles[i], u.size[1], shape.box_rows, &v_full[s], landed, phase);
+            if (!ok) break;
         }
         if (!ok) {
             misc[1] = 1;
-            if (lane == 0) {  // no copy stays in flight
-                ptx::mbar_wait(rows_full, 0);
-                for (uint32_t j = i > kDqtStages ? i - kDqtStages : 0; j < i; ++j) ptx::mbar_wait(&full[j % kDqtStages], (j / kDqtStages) & 1u);
+            if (lane == 0)  // no copy stays in flight
+                for (uint32_t j = i > kDqStages ? i - kDqStages : 0; j <= i && j < units; ++j) {
+                    ptx::mbar_wait(&k_full[j % kDqStages], (j / kDqStages) & 1u);
+                    ptx::mbar_wait(&v_full[j % kDqStages], (j / kDqStages) & 1u);
+                }
+        }
+    } else if (warp == kDqWarps + 1) {
+        if (lane == 0) {
+            constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, 128, 64);
+            const uint64_t k_k = tc::desc_k(ptx::smem_u32(smem) + S::kKeys), v_k = tc::desc_k(ptx::smem_u32(smem) + S::kValues);
+            ok = ptx::mbar_wait(rows_in, 0);
+            for (uint32_t i = 0; ok && i < units; ++i) {
+                const uint32_t s = i % kDqStages, parity = (i / kDqStages) & 1u, at = s * (S::kTile >> 4), buffer = tmem + (i & 1u) * kDqBuffer;
+                // the buffer held dS two tiles ago
+                if (!(ok = ptx::mbar_wait(&k_full[s], parity) && ptx::mbar_wait(&v_full[s], parity) && (i < 2 || ptx::mbar_wait(&summed[(i - 2) % kDqStages], ((i - 2) / kDqStages) & 1u)))) break;
+                tc::fence_after();
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) tc::mma_ta(buffer, tmem + kDqQ + d * 8, k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id, d != 0);
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) tc::mma_ta(buffer + 64, tmem + kDqDo + d * 8, v_k + (at + (d >> 2) * 512 + (d & 3) * 2), id, d != 0);
+                tc::commit(&scored[s]);
             }
-        } else if (!units && lane == 0)
-            ok = ptx::mbar_wait(rows_full, 0);
-    } else if (warp == kDqtWarps + 1) {
-        if (lane == 0 && units) {
-            constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-            constexpr uint32_t id_s = tc::idesc(bf16, 128, 64), id_q = tc::idesc(bf16, 128, DP, false, true);
-            const uint32_t base = ptx::smem_u32(smem);
-            const uint64_t q_k = tc::desc_k(base + S::kQ), k_k = tc::desc_k(base + S::kRing), k_mn = tc::desc_mn(base + S::kRing, 64 * 128);
-            constexpr uint32_t kDoAt = S::kDo >> 4, kValuesAt = (S::kHalves * 64 * 128) >> 4;
-            ok = ptx::mbar_wait(rows_full, 0);
-            uint32_t scores = 0, sums = 0;
-            for (uint32_t idle = 0; ok && sums < units;) {
-                if (sums < scores && ptx::mbar_test(&formed[sums & 1u], (sums >> 1) & 1u)) {
-                    tc::fence_after();
-                    const uint32_t s = sums % kDqtStages, at = s * (S::kStage >> 4);
+            if (!ok) misc[1] = 1;
+        }
+    } else if (warp == kDqWarps + 2) {
+        if (lane == 0) {
+            constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, 128, DP, false, true);
+            const uint64_t k_mn = tc::desc_mn(ptx::smem_u32(smem) + S::kKeys, 64 * 128);
+            for (uint32_t i = 0; i < units; ++i) {
+                const uint32_t s = i % kDqStages, at = s * (S::kTile >> 4), ds = tmem + (i & 1u) * kDqBuffer;
+                if (!(ok = ptx::mbar_wait(&formed[s], (i / kDqStages) & 1u))) break;
+                tc::fence_after();
+                // the two threads of a row leave 16 columns each, where they read S
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kDqtSum, tmem + kDqtDs + (sums & 1u) * 32 + k * 8, k_mn + (at + k * 128), id_q, sums || k);
-                    tc::commit(&empty[s]);
-                    tc::commit(summed);
-                    ++sums;
-                    idle = 0;
-                } else if (scores < units && scores < sums + 2 && ptx::mbar_test(&full[scores % kDqtStages], (scores / kDqtStages) & 1u)) {
-                    tc::fence_after();
-                    const uint32_t at = scores % kDqtStages * (S::kStage >> 4), buffer = tmem + (scores & 1u) * kDqtBuffer;
-#pragma unroll
-                    for (int d = 0; d < DP / 16; ++d) tc::mma(buffer, q_k + ((d >> 2) * 1024 + (d & 3) * 2), k_k + (at + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
-#pragma unroll
-                    for (int d = 0; d < DP / 16; ++d) tc::mma(buffer + 64, q_k + (kDoAt + (d >> 2) * 1024 + (d & 3) * 2), k_k + (at + kValuesAt + (d >> 2) * 512 + (d & 3) * 2), id_s, d != 0);
-                    tc::commit(&scored[scores & 1u]);
-                    ++scores;
-                    idle = 0;
-                } else if (++idle == kTcPolls)
-                    ok = false;
+                for (int k = 0; k < 4; ++k) tc::mma_ta(tmem + kDqSum, ds + (k >> 1) * 32 + (k & 1) * 8, k_mn + (at + k * 128), id, i || k);
+                tc::commit(&summed[s]);
             }
             if (!ok) misc[1] = 1;
         }
     } else {
-        const float *shares = reinterpret_cast<const float *>(smem + S::kDelta);
+        const uint32_t r = threadIdx.x & 127, half = threadIdx.x >> 7, q = r / shape.heads, h = r % shape.heads, head = kv * group + head0 + h;
+        const bool real = q < queries && h < heads;
+        const uint32_t tq = real ? t0 + q : t0, th = real ? head : kv * group;  // rows that are none read a row that is
+        const uint64_t row = ((uint64_t)b * a.queries + tq) * a.heads + th, stat = ((uint64_t)b * a.heads + th) * a.queries + tq;
+        const uint32_t lanes_in = tmem + (((warp & 3) * 32) << 16), dims = !real || a.dim <= half * kHalfDims ? 0u : min(a.dim - half * kHalfDims, kHalfDims);
+        const T *dout = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)tq * a.do_query + (int64_t)th * a.do_head + half * kHalfDims;
+        row_to_tmem<T, DP / 16>(lanes_in + kDqQ + half * (DP / 4), static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)tq * a.q_query + (int64_t)th * a.q_head + half * kHalfDims, dims);
+        row_to_tmem<T, DP / 16>(lanes_in + kDqDo + half * (DP / 4), dout, dims);
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(rows_in);
+        // delta = <dout, out>, while the first tiles are on their way
+        float part = 0.f;
+        const T *out = static_cast<const T *>(a.out) + row * a.dim + half * kHalfDims;
+#pragma unroll
+        for (uint32_t x = 0; x < kHalfDims / 8; ++x)
+            if (8 * x < dims) {
+                const Pack<T, 8> o = load_pack<T, 8>(out + 8 * x), g = load_pack<T, 8>(dout + 8 * x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) part = fmaf(to_f32(o.x[j]), to_f32(g.x[j]), part);
+            }
+        float *shares = reinterpret_cast<float *>(smem + S::kDelta);
+        shares[half * 128 + r] = part;
+        asm volatile("bar.sync 1, %0;" ::"n"(kDqWarps * 32) : "memory");
         const float delta = shares[r] + shares[128 + r], lse = real ? a.lse[stat] * kLog2e : 0.f, scale_log2 = a.scale * kLog2e;
         if (real && half == 0) a.delta[stat] = delta;
         const uint32_t lanes = tmem + (((warp & 3) * 32) << 16);
         for (uint32_t i = 0; i < units; ++i) {
             const uint64_t both = real ? u.seen(i, q, a.block) : 0ull;
             const uint32_t seen = half ? (uint32_t)(both >> 32) : (uint32_t)both;
-            const uint32_t buffer = lanes + (i & 1u) * kDqtBuffer + half * 32;
-            if (!(ok = ptx::mbar_wait_warp(&scored[i & 1u], (i >> 1) & 1u))) break;
+            const uint32_t s = i % kDqStages, buffer = lanes + (i & 1u) * kDqBuffer + half * 32;
+            if (!(ok = ptx::mbar_wait_warp(&scored[s], (i / kDqStages) & 1u))) break;
             tc::fence_after();
             uint32_t ds[16];
             if (__any_sync(~0u, seen != 0)) {
@@ -229,15 +243,13 @@ __global__ void __launch_bounds__(kDqtThreads, 1)
                 for (int c = 0; c < 16; ++c) ds[c] = 0;
             }
             __syncwarp();
-            tc::st16(lanes + kDqtDs + (i & 1u) * 32 + half * 16, ds);
+            tc::st16(buffer, ds);
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&formed[i & 1u]);
+            if (lane == 0) ptx::mbar_arrive(&formed[s]);
         }
-        // the last two, in order: a parity names the one before the last as well as the one to come
-        if (ok && units > 1) ok = ptx::mbar_wait_warp(summed, (units - 2) & 1u);
-        if (ok && units) ok = ptx::mbar_wait_warp(summed, (units - 1) & 1u);
+        if (ok && units) ok = ptx::mbar_wait_warp(&summed[(units - 1) % kDqStages], ((units - 1) / kDqStages) & 1u);
         tc::fence_after();
         if (!ok) misc[1] = 1;
         T *dst = static_cast<T *>(a.dq) + row * a.dim;
@@ -246,7 +258,7 @@ __global__ void __launch_bounds__(kDqtThreads, 1)
         for (uint32_t c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
             uint32_t o[32];
             if (units) {
-                tc::ld32(lanes + kDqtSum + c, o);
+                tc::ld32(lanes + kDqSum + c, o);
                 tc::wait_ld();
             }
 #pragma unroll
@@ -273,7 +285,7 @@ __global__ void __launch_bounds__(kDqtThreads, 1)
     if (threadIdx.x == 0 && misc[1]) atomicExch(&g_status, 1u);
     if (warp == 0) {
         tc::fence_after();
-        tc::dealloc(tmem, kDqtCols);
+        tc::dealloc(tmem, kDqCols);
     }
 }
 
@@ -794,19 +806,17 @@ template <class T, int DP> cudaError_t launch_dq(const AttentionArgs &a, cudaStr
     TcShape shape = tc_shape(a.heads / a.kv_heads, 64);
     uint32_t bytes = 0;  // fewer queries where their lists are too long
     for (;; shape.queries /= 2)
-        if ((bytes = DqtSmem<DP>::kLists + TileUnion::bytes(shape.queries, a.count, a.block, a.keys)) <= kSmemMost || shape.queries == 1) break;
-    CUtensorMap k_map{}, v_map{}, q_map, do_map;
+        if ((bytes = DqSmem<DP>::kLists + TileUnion::bytes(shape.queries, a.count, a.block, a.keys)) <= kSmemMost || shape.queries == 1) break;
+    CUtensorMap k_map{}, v_map{};
     cudaError_t e = cudaSuccess;
     if (a.keys) {
         e = tc::make_map(&k_map, bf16, a.k, a.dim, a.kv_heads, a.keys, a.batch, a.k_head, a.k_key, a.k_batch, 64);
         if (e == cudaSuccess) e = tc::make_map(&v_map, bf16, a.v, a.dim, a.kv_heads, a.keys, a.batch, a.v_head, a.v_key, a.v_batch, 64);
     }
-    if (e == cudaSuccess) e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, shape.queries, shape.heads);
-    if (e == cudaSuccess) e = tc::make_map(&do_map, bf16, a.dout, a.dim, a.heads, a.queries, a.batch, a.do_head, a.do_query, a.do_batch, shape.queries, shape.heads);
     if (e == cudaSuccess) e = allow_dynamic_smem<block_attention_dq_kernel<T, DP>>(kSmemMost);
     if (e != cudaSuccess) return e;
     const dim3 grid((a.queries + shape.queries - 1) / shape.queries, a.kv_heads * shape.chunks, a.batch);
-    return launch_overlapped(block_attention_dq_kernel<T, DP>, grid, dim3(kDqtThreads), bytes, s, k_map, v_map, q_map, do_map, a, shape);
+    return launch_overlapped(block_attention_dq_kernel<T, DP>, grid, dim3(kDqThreads), bytes, s, k_map, v_map, a, shape);
 }
 
 template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count, cudaStream_t s)
