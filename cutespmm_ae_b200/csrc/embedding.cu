@@ -64,7 +64,7 @@ template <class T, int V> __global__ void __launch_bounds__(kWarps * 32) embeddi
 
 constexpr int kMaxDigitBits = 9, kMaxBins = 1 << kMaxDigitBits;
 constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32;
-constexpr uint32_t kMaxSortBlocks = 512;
+constexpr uint32_t kMaxSortBlocks = 256;
 
 struct SortArgs {
     const void *tokens;  // first pass: keys are made from the tokens
@@ -240,33 +240,42 @@ template <class T, int V> struct Rows {
         clear();
     }
     // Adds the rows of positions [b, e) in order; where EACH, a row of dtable is written at the end of each token, else the sum stays.
+    // The lanes of a warp hold 32 positions' keys and places, the next 32 on their way, so that loads of rows wait for no index.
     template <bool EACH> __device__ void walk(uint32_t b, uint32_t e)
     {
+        if (b >= e) return;
         const T *src = static_cast<const T *>(a.e.src) + c;
-        uint32_t row = EACH && b < e ? a.keys[b] : 0u;
-        for (uint32_t i = b; i < e; i += kRowsInFlight) {
-            Pack<T, V> p[kRowsInFlight];
-            uint32_t key[kRowsInFlight];
+        const uint32_t lane = threadIdx.x & 31;
+        uint32_t place = b + lane < e ? a.order[b + lane] : 0u, key = EACH && b + lane < e ? a.keys[b + lane] : 0u;
+        uint32_t row = __shfl_sync(~0u, key, 0);
+        for (uint32_t w = b; w < e; w += 32) {
+            const uint32_t n = min(32u, e - w);
+            const uint32_t next_place = w + 32 + lane < e ? a.order[w + 32 + lane] : 0u, next_key = EACH && w + 32 + lane < e ? a.keys[w + 32 + lane] : 0u;
+            for (uint32_t x = 0; x < n; x += kRowsInFlight) {
+                Pack<T, V> p[kRowsInFlight];
 #pragma unroll
-            for (int u = 0; u < kRowsInFlight; ++u)
-                if (i + u < e) {
-                    if (EACH) key[u] = a.keys[i + u];
-                    if (on) p[u] = load_pack<T, V>(src + a.order[i + u] * a.e.ld_src);
+                for (int u = 0; u < kRowsInFlight; ++u) {
+                    const uint32_t at = __shfl_sync(~0u, place, x + u);
+                    if (on && x + u < n) p[u] = load_pack<T, V>(src + at * a.e.ld_src);
                 }
 #pragma unroll
-            for (int u = 0; u < kRowsInFlight; ++u)
-                if (i + u < e) {
-                    if (EACH && key[u] != row) {
+                for (int u = 0; u < kRowsInFlight; ++u) {
+                    const uint32_t token = __shfl_sync(~0u, key, x + u);
+                    if (x + u >= n) break;
+                    if (EACH && token != row) {
                         flush(row);
-                        row = key[u];
+                        row = token;
                     }
                     if (on) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) acc[j] += to_f32(p[u].x[j]);
                     }
                 }
+            }
+            place = next_place;
+            key = next_key;
         }
-        if (EACH && b < e) flush(row);
+        if (EACH) flush(row);
     }
 };
 
@@ -406,8 +415,8 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs &a, void *workspace, int s
         p.token_bytes = a.token_bytes;
         p.vocab = a.vocab;
         p.n = sum.n;
-        // 256 keys a warp, more where that would make too many blocks
-        p.per_warp = 256;
+        // 64 keys a warp: a pass is a chain of latencies; more where that would make too many blocks (65536 tokens 30 us a pass with 256)
+        p.per_warp = 64;
         while ((a.count + (uint64_t)p.per_warp * kSortWarps - 1) / ((uint64_t)p.per_warp * kSortWarps) > kMaxSortBlocks) p.per_warp *= 2;
         const unsigned blocks = (unsigned)((a.count + (uint64_t)p.per_warp * kSortWarps - 1) / ((uint64_t)p.per_warp * kSortWarps));
         p.bins = 1u << digit;
