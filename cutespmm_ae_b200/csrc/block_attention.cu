@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
 // order of the warps, first inside a thread block, then over the cluster through distributed shared memory: no scratch, no counters, one
 // launch.  Bound: HBM (the named blocks once) in batches, a chain of latencies for one sequence.
 constexpr int kSplitWarps = 4, kSplitUnit = 16;
-template <int DP> constexpr int kSplitStages = DP == 128 ? 4 : 8;
+template <int DP> constexpr int kSplitStages = DP == 128 ? 2 : 4;  // 64 KB of keys and values: three thread blocks share an SM
 constexpr uint32_t kSplitCount = 128;  // most blocks of a query
 
 __device__ __forceinline__ void cluster_sync()
@@ -426,8 +426,9 @@ template <int DP, int NT> struct SplitSmem {
     static constexpr int kStage = kUnitBytes<DP, kSplitUnit>;
     static constexpr int kRings = kSplitWarps * kSplitStages<DP> * kStage;
     static constexpr int kPitch = DP + 4;                                      // floats of a column of a partial result
-    static constexpr int kPartial = kRings;                                    // per warp 8 NT columns; the thread block's own join lies in warp 0's
-    static constexpr int kStats = kPartial + kSplitWarps * 8 * NT * kPitch * 4;  // per warp and column: maximum, sum
+    static constexpr int kRing = kSplitStages<DP> * kStage;                    // of a warp; its partial result takes the ring's place
+    static_assert(8 * NT * kPitch * 4 <= kRing, "a warp's partial result fits its ring");
+    static constexpr int kStats = kRings;                                      // per warp and column: maximum, sum
     static constexpr int kBars = kStats + kSplitWarps * 8 * NT * 8;
     static constexpr int kList = kBars + kSplitWarps * kSplitStages<DP> * 8;
     static constexpr int kBytes = kList + kSplitCount * 8 + 16;
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
     const uint32_t per_block = a.block / kSplitUnit, units = total * per_block;
     const uint32_t walkers = ranks * kSplitWarps, me = warp * ranks + rank;  // neighbouring units go to different thread blocks
     const uint32_t mine_units = units > me ? (units - me + walkers - 1) / walkers : 0u;
-    unsigned char *ring = smem + warp * STAGES * S::kStage;
+    unsigned char *ring = smem + warp * S::kRing;
     auto issue = [&](uint32_t i) {
         const uint32_t n = me + i * walkers;
         int row, outer;
@@ -539,7 +540,9 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
     }
 
     // this warp's columns: maximum, sum and O, not divided
-    float *partial = reinterpret_cast<float *>(smem + S::kPartial), *stats = reinterpret_cast<float *>(smem + S::kStats);
+    __syncwarp();  // every lane is done with the ring
+    auto partial = [&](uint32_t w, uint32_t col) { return reinterpret_cast<float *>(smem + w * S::kRing) + col * S::kPitch; };
+    float *stats = reinterpret_cast<float *>(smem + S::kStats);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         tile[j].finish_sum();
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
                 stats[(warp * 8 * NT + col) * 2] = tile[j].top[h];
                 stats[(warp * 8 * NT + col) * 2 + 1] = tile[j].sum[h];
             }
-            float *o = partial + (warp * 8 * NT + col) * S::kPitch + lane / 4;
+            float *o = partial(warp, col) + lane / 4;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 o[d * 16] = tile[j].o[d][h];
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
             for (uint32_t w = 0; w < (uint32_t)kSplitWarps; ++w) {
                 const uint32_t c = w * 8 * NT + col;
                 const float f = tc::exp2_fast(peer_load(stats + c * 2, r) - base);
-                const float4 x = peer_load4(partial + c * S::kPitch + d, r);
+                const float4 x = peer_load4(partial(w, col) + d, r);
                 sum = fmaf(f, peer_load(stats + c * 2 + 1, r), sum);
                 o.x = fmaf(f, x.x, o.x);
                 o.y = fmaf(f, x.y, o.y);
@@ -600,9 +603,10 @@ template <class T, int DP, int NT> cudaError_t launch_split(const CUtensorMap &k
     if (e != cudaSuccess) return e;
     const uint32_t group = a.heads / a.kv_heads, chunks = (group + 8 * NT - 1) / (8 * NT);
     const uint64_t rows = (uint64_t)a.batch * a.queries * a.kv_heads * chunks, units = (uint64_t)a.count * (a.block / kSplitUnit);
-    // thread blocks per query: as many as keep the machine busy, while each warp has two pieces of 16 keys
+    // thread blocks per query: enough for a few rounds of three on each SM, so that the last round costs little, while a warp has four pieces
+    // of 16 keys (two where the machine would not be full otherwise)
     uint32_t ranks = 1;
-    while (ranks < 8 && rows * ranks < (uint64_t)sm_count && units >= 4ull * ranks * kSplitWarps) ranks *= 2;
+    while (ranks < 8 && rows * ranks < 12ull * sm_count && units >= (rows * ranks < (uint64_t)sm_count ? 4ull : 8ull) * ranks * kSplitWarps) ranks *= 2;
     cudaLaunchAttribute attr[2]{};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -156,23 +156,14 @@ template <class T> __global__ void __launch_bounds__(kScoreThreads) block_scores
 
 // ---- selection ---------------------------------------------------------------------------------------------------------
 // WARPS warps take one row of scores, 32 * R consecutive ones each, in registers as unsigned integers of the same order (0: not to be
-// chosen; all ones: chosen in any case).  The count-th largest is found bit by bit from the top -- how many are at least this
-// candidate? -- and the search ends as soon as a candidate leaves exactly `count`.  Then the chosen indices are written in ascending
-// order, equal scores from the lowest index on.  Bound: HBM in large calls (the visible scores once), latency in small ones.
-template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) select_blocks_kernel(SelectArgs a, uint64_t rows)
+// chosen; all ones: chosen in any case).  The count-th largest is found by halving an interval of integers -- how many are at least this
+// candidate? -- until a candidate leaves exactly `count`; with up to 32 to choose the interval begins at the least of the lanes' largest
+// keys, of which there are 32, and takes some eight halvings instead of twenty from the top bit down (16384 x 4 rows of 256, 16 to choose:
+// 58 us that way).  Then the chosen indices are written in ascending order, equal scores from the lowest index on.  Bound: instructions in large calls,
+// latency in small ones.
+template <int R, int WARPS> __device__ __forceinline__ void select_row(const SelectArgs &a, const float *src, uint32_t n, int32_t *out, uint32_t (*counts)[2])
 {
-    constexpr int kRowsPerBlock = WARPS == 1 ? 4 : 1;
-    __shared__ uint32_t counts[WARPS][2];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = WARPS == 1 ? 0 : warp;
-    ptx::grid_wait();
-    ptx::grid_release();
-    const uint64_t row = (uint64_t)blockIdx.x * kRowsPerBlock + (WARPS == 1 ? warp : 0);
-    if (row >= rows) return;
-    const uint32_t t = (uint32_t)(row % a.queries), bh = (uint32_t)(row / a.queries), b = bh / a.kv_heads;
-    const int64_t see = a.visible ? a.visible[(uint64_t)b * a.queries + t] : (int64_t)a.keys - a.queries + 1 + t;
-    const uint32_t visible = (uint32_t)min(max(see, (int64_t)0), (int64_t)a.keys);
-    const uint32_t n = min((visible + a.block - 1) / a.block, a.blocks);
-    const float *src = a.scores + (int64_t)b * a.s_batch + (int64_t)(bh % a.kv_heads) * a.s_head + (int64_t)t * a.s_query;
     const uint32_t i0 = part * R * 32 + lane;
     uint32_t key[R];
     uint32_t any = 0;
@@ -201,25 +192,54 @@ template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 :
         }
         return v;
     };
-    uint32_t limit = 1;     // chosen: every key above it, and the first `ties` that equal it
-    uint32_t ties = ~0u;
+    uint32_t limit = 0;     // chosen: every key above it, and the first `ties` that equal it (never keys of 0)
+    uint32_t ties = 0;
     if (total(any) > a.count) {
-        limit = 0;
-        bool exact = false;
-        for (int bit = 31; bit >= 0 && !exact; --bit) {
-            const uint32_t cand = limit | (1u << bit);
-            uint32_t c = 0;
+        uint32_t top = 0, least = 0;
 #pragma unroll
-            for (int r = 0; r < R; ++r) c += key[r] >= cand;
-            c = total(c);
-            if (c >= a.count) limit = cand;
-            exact = c == a.count;
+        for (int r = 0; r < R; ++r) top = max(top, key[r]);
+        if (a.count <= 32) least = __reduce_min_sync(~0u, top);
+        top = __reduce_max_sync(~0u, top);
+        if constexpr (WARPS > 1) {
+            __syncthreads();
+            if (lane == 0) {
+                counts[warp][0] = top;
+                counts[warp][1] = least;
+            }
+            __syncthreads();
+            least = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                top = max(top, counts[w][0]);
+                least = max(least, counts[w][1]);  // any warp's 32 lanes will do
+            }
         }
-        if (!exact) {
-            uint32_t c = 0;
+        // at least `lo` are count keys and more, at least `hi` are fewer than count, or exactly that many (hi found)
+        uint32_t lo = max(least, 1u), hi = top;
+        uint32_t c = 0;
 #pragma unroll
-            for (int r = 0; r < R; ++r) c += key[r] > limit;
-            ties = a.count - total(c);
+        for (int r = 0; r < R; ++r) c += key[r] >= hi;
+        uint32_t above = total(c);  // keys of at least hi
+        if (above > a.count) {      // so many equal ones at the top
+            lo = hi;
+            above = 0;
+        } else
+            while (above != a.count && hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                c = 0;
+#pragma unroll
+                for (int r = 0; r < R; ++r) c += key[r] >= mid;
+                c = total(c);
+                if (c <= a.count) {
+                    hi = mid;
+                    above = c;
+                } else
+                    lo = mid;
+            }
+        if (above == a.count) limit = hi - 1;
+        else {
+            limit = lo;
+            ties = a.count - above;
         }
     }
     uint32_t before = 0, ties_before = 0;  // chosen, and equal to the limit, at lower indices
@@ -228,7 +248,7 @@ template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 :
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             above += key[r] > limit;
-            equal += key[r] == limit;
+            equal += ties && key[r] == limit;
         }
         above = __reduce_add_sync(~0u, above);
         equal = __reduce_add_sync(~0u, equal);
@@ -244,19 +264,49 @@ template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 :
         }
         before += min(ties_before, ties);
     }
-    int32_t *out = a.out + row * a.count;
     const uint32_t below = (1u << lane) - 1u;
+    if (ties) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const uint32_t equal = __ballot_sync(~0u, key[r] == limit);
-        const bool tie = key[r] == limit && ties_before + __popc(equal & below) < ties;
-        const uint32_t chosen = __ballot_sync(~0u, key[r] > limit || tie);
-        if ((chosen >> lane) & 1u) out[before + __popc(chosen & below)] = (int32_t)(i0 + r * 32);
-        before += __popc(chosen);
-        ties_before += __popc(equal);
+        for (int r = 0; r < R; ++r) {
+            const uint32_t equal = __ballot_sync(~0u, key[r] == limit);
+            const uint32_t chosen = __ballot_sync(~0u, key[r] > limit || (key[r] == limit && ties_before + __popc(equal & below) < ties));
+            if ((chosen >> lane) & 1u) out[before + __popc(chosen & below)] = (int32_t)(i0 + r * 32);
+            before += __popc(chosen);
+            ties_before += __popc(equal);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool mine = key[r] > limit;
+            const uint32_t chosen = __ballot_sync(~0u, mine);
+            if (mine) out[before + __popc(chosen & below)] = (int32_t)(i0 + r * 32);
+            before += __popc(chosen);
+        }
     }
     if (part == WARPS - 1)
         for (uint32_t i = before + lane; i < a.count; i += 32) out[i] = -1;
+}
+
+template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) select_blocks_kernel(SelectArgs a)
+{
+    constexpr int kRowsPerBlock = WARPS == 1 ? 4 : 1;
+    __shared__ uint32_t counts[WARPS][2];
+    ptx::grid_wait();
+    ptx::grid_release();
+    const uint32_t t = blockIdx.x * kRowsPerBlock + (WARPS == 1 ? threadIdx.x >> 5 : 0), bh = blockIdx.y, b = bh / a.kv_heads;
+    if (t >= a.queries) return;
+    const int64_t see = a.visible ? a.visible[(uint64_t)b * a.queries + t] : (int64_t)a.keys - a.queries + 1 + t;
+    const uint32_t visible = (uint32_t)min(max(see, (int64_t)0), (int64_t)a.keys);
+    const uint32_t n = min((visible + a.block - 1) / a.block, a.blocks);
+    const float *src = a.scores + (int64_t)b * a.s_batch + (int64_t)(bh % a.kv_heads) * a.s_head + (int64_t)t * a.s_query;
+    int32_t *out = a.out + ((uint64_t)bh * a.queries + t) * a.count;
+    // a row that sees a half or a quarter of the blocks takes as many instructions less
+    if constexpr (WARPS == 1 && R >= 4) {
+        if (n <= R * 8) select_row<R / 4, 1>(a, src, n, out, counts);
+        else if (n <= R * 16) select_row<R / 2, 1>(a, src, n, out, counts);
+        else select_row<R, 1>(a, src, n, out, counts);
+    } else
+        select_row<R, WARPS>(a, src, n, out, counts);
 }
 
 }  // namespace
@@ -288,8 +338,9 @@ cudaError_t launch_select_blocks(const SelectArgs &a, int sm_count, cudaStream_t
 {
     const uint64_t rows = (uint64_t)a.batch * a.kv_heads * a.queries;
     if (!rows || !a.count) return cudaSuccess;
-    auto one = [&](auto kernel) { return launch_overlapped(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, a, rows); };
-    auto eight = [&](auto kernel) { return launch_overlapped(kernel, dim3((unsigned)rows), dim3(256), 0, s, a, rows); };
+    const unsigned heads = a.batch * a.kv_heads;
+    auto one = [&](auto kernel) { return launch_overlapped(kernel, dim3((a.queries + 3) / 4, heads), dim3(128), 0, s, a); };
+    auto eight = [&](auto kernel) { return launch_overlapped(kernel, dim3(a.queries, heads), dim3(256), 0, s, a); };
     // eight warps a row where there are too few rows to fill the machine with a warp each, or too many scores for one warp's registers
     if (a.blocks <= 1024 && (a.blocks <= 32 || rows > (uint64_t)sm_count * 8)) {
         if (a.blocks <= 32) return one(select_blocks_kernel<1, 1>);

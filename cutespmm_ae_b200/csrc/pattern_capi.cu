@@ -165,7 +165,7 @@ int cutespmm_select_blocks(const float *scores_dev, const int64_t s_strides[3], 
     if ((uint64_t)first + last > count) return refuse(CUTESPMM_EINVAL, "first + last must not exceed count");
     if (blocks > 16384) return refuse(CUTESPMM_EUNSUPPORTED, "at most 16384 blocks");
     if (keys >> 28 || queries >> 28 || count >> 16) return refuse(CUTESPMM_EUNSUPPORTED, "too many keys, queries or blocks per query");
-    if (((uint64_t)batch * kv_heads * queries) >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "more than 2^31 - 1 rows of scores");
+    if (!fits_grid((uint64_t)batch * kv_heads)) return refuse(CUTESPMM_EUNSUPPORTED, "batch * kv_heads must be at most 65535");
     if (batch && kv_heads && queries && count && ((blocks && (!scores_dev || !s_strides)) || !blocks_dev)) return refuse(CUTESPMM_EINVAL, "scores, strides or blocks is NULL");
     int dev = -1, sms = 0, st;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
