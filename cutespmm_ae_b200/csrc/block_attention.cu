@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 }
 
 // ---- a tile of queries -------------------------------------------------------------------------------------------------
-// 128 rows -- up to 32 neighbouring queries with all heads of a group (or a chunk of them) -- against the union of the tiles of 64 keys that they name:
+// 128 rows -- neighbouring queries with all heads of a group (or a chunk of them) -- against the union of the tiles of 64 keys that they name:
 //     S = Q K^T (128 x 64, two buffers in tensor memory);  P from registers back into S's columns as 16-bit operand;  O += P V.
 // Warps 0-3 hold a row each lane (a row's maximum and sum need no other lane), warp 4 loads, warp 5 issues S, warp 6 O: one warp for both
 // spent a third of a tile's time between them.
@@ -626,7 +626,7 @@ template <class T, int DP, int NT> cudaError_t launch_split(const CUtensorMap &k
 template <class T, int DP> cudaError_t launch_tile(const CUtensorMap &k_map, const CUtensorMap &v_map, const AttentionArgs &a, uint32_t box_rows, cudaStream_t s)
 {
     TcShape shape = tc_shape(a.heads / a.kv_heads, box_rows);
-    uint32_t bytes = 0;  // fewer queries where their lists are too long (more than 100 blocks of 16 for each of 32 queries)
+    uint32_t bytes = 0;  // fewer queries where their lists are too long (tens of blocks for each of 128 queries)
     for (;; shape.queries /= 2)
         if ((bytes = TcSmem<DP>::kLists + TileUnion::bytes(shape.queries, a.count, a.block, a.keys)) <= kSmemMost || shape.queries == 1) break;
     CUtensorMap q_map;

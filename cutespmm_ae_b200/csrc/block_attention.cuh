@@ -12,8 +12,8 @@
 
 namespace cutespmm {
 
-constexpr uint32_t kTileQueries = 32;  // at most: a bit of a word each
-constexpr uint32_t kHeadChunk = 64;    // query heads of a group that one block of threads takes, at most
+constexpr uint32_t kTileQueries = 128;  // at most: a row each
+constexpr uint32_t kHeadChunk = 64;     // query heads of a group that one block of threads takes, at most
 constexpr float kLog2e = 1.4426950408889634f;
 
 // How many keys query t of sequence b sees.
@@ -52,9 +52,9 @@ __host__ __device__ inline uint32_t tiles_of_block(uint32_t block) { return bloc
 // The union of the tiles of keys that hold a block which some of `queries` queries from t0 on name, ascending; for each part (block) of
 // each tile a bit per query that names it.
 struct TileUnion {
-    uint32_t *tiles, *names;  // names: slot * parts + part
+    uint32_t *tiles, *names;  // names: (slot * parts + part) * sets + query / 32
     uint32_t *visible, *bits, *before, *size;
-    uint32_t parts;
+    uint32_t parts, sets;     // sets of 32 queries
 
     static __host__ __device__ uint32_t words(uint32_t keys) { return (keys + kKeyTile * 32 - 1) / (kKeyTile * 32); }
     static __host__ __device__ uint32_t slots(uint32_t queries, uint32_t count, uint32_t block, uint32_t keys)
@@ -64,15 +64,16 @@ struct TileUnion {
     }
     static __host__ __device__ uint32_t bytes(uint32_t queries, uint32_t count, uint32_t block, uint32_t keys)
     {
-        return (slots(queries, count, block, keys) * (1 + parts_of_tile(block)) + kTileQueries + 2 * words(keys) + 4) * 4;
+        return (slots(queries, count, block, keys) * (1 + parts_of_tile(block) * ((queries + 31) / 32)) + queries + 2 * words(keys) + 4) * 4;
     }
     __device__ TileUnion(unsigned char *p, uint32_t queries, const AttentionArgs &a)
     {
         uint32_t *w = reinterpret_cast<uint32_t *>(p);
         parts = parts_of_tile(a.block);
+        sets = (queries + 31) / 32;
         size = w;
         visible = w + 4;
-        bits = visible + kTileQueries;
+        bits = visible + queries;
         before = bits + words(a.keys);
         tiles = before + words(a.keys);
         names = tiles + slots(queries, a.count, a.block, a.keys);
@@ -82,7 +83,7 @@ struct TileUnion {
     {
         const uint32_t w = words(a.keys), n = queries * a.count, per = tiles_of_block(a.block);
         const int32_t *src = a.blocks + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0) * a.count;
-        const uint32_t most_names = slots(queries, a.count, a.block, a.keys) * parts;
+        const uint32_t most_names = slots(queries, a.count, a.block, a.keys) * parts * sets;
         for (uint32_t i = threadIdx.x; i < w; i += blockDim.x) bits[i] = 0;
         for (uint32_t i = threadIdx.x; i < most_names; i += blockDim.x) names[i] = 0;
         for (uint32_t i = threadIdx.x; i < queries; i += blockDim.x) visible[i] = visible_keys(a, b, t0 + i);
@@ -110,7 +111,7 @@ struct TileUnion {
                 if (i + threadIdx.x < w) before[i + threadIdx.x] = sum + scan - mine;
                 sum += __shfl_sync(~0u, scan, 31);
             }
-            if (threadIdx.x < queries) most = visible[threadIdx.x];
+            for (uint32_t i = threadIdx.x; i < queries; i += 32) most = max(most, visible[i]);
             most = __reduce_max_sync(~0u, most);
             if (threadIdx.x == 0) {
                 size[0] = sum;
@@ -122,7 +123,7 @@ struct TileUnion {
             each(i, i == threadIdx.x ? mine : src[i], visible[i / a.count], [&](uint32_t tile, uint32_t part, uint32_t q) {
                 const uint32_t at = before[tile >> 5] + __popc(bits[tile >> 5] & ((1u << (tile & 31)) - 1u));
                 tiles[at] = tile;
-                atomicOr(&names[at * parts + part], 1u << q);
+                atomicOr(&names[(at * parts + part) * sets + (q >> 5)], 1u << (q & 31));
             });
         __syncthreads();
     }
@@ -131,10 +132,11 @@ struct TileUnion {
     {
         const int64_t limit = (int64_t)visible[q] - (int64_t)tiles[slot] * kKeyTile;
         const uint64_t below = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1ull : 0ull;
-        if (parts == 1) return (names[slot] >> q) & 1u ? below : 0ull;
+        const uint32_t *word = names + slot * parts * sets + (q >> 5), bit = 1u << (q & 31);
+        if (parts == 1) return *word & bit ? below : 0ull;
         uint64_t named = 0;
         for (uint32_t i = 0; i < parts; ++i)
-            if ((names[slot * parts + i] >> q) & 1u) named |= ((1ull << block) - 1ull) << (i * block);
+            if (word[i * sets] & bit) named |= ((1ull << block) - 1ull) << (i * block);
         return named & below;
     }
 };
