@@ -56,101 +56,185 @@ template <class T> __global__ void __launch_bounds__(kMeanWarps * 32) block_mean
 
 // ---- scores ------------------------------------------------------------------------------------------------------------
 // scores[t, n] = sum over the heads h of a group of q[t, h] . means[n]: one product with heads and dims side by side as K, so that the
-// sum over heads costs no additions of its own and q is read once.  Per block 128 queries x up to 256 means; the means stay in shared
-// memory (they are the same operand for every head), q arrives through a ring of TMA tiles, the products of 16-bit values are exact and
-// are added in fp32 in tensor memory.  Bound: HBM (q and the scores).
-constexpr int kScoreRows = 128, kScoreCols = 256, kScoreStages = 3;
+// sum over heads costs no additions of its own; the products of 16-bit values are exact and are added in fp32 in tensor memory.  A thread block per
+// SM walks jobs of 128 queries x up to 512 means: q comes from memory once, through a ring of TMA tiles, each multiplied with two tiles of 256 means that
+// stay in shared memory (they are the same operand for every head).  Eight warps write the two accumulators out.  With up to 256 means a job uses one
+// accumulator, in turn, and the ring is twice as deep.  Bound: HBM (q and the scores) and the tensor cores about equally (32768 queries, 32 heads, 512 blocks:
+// 82 and 70 us); it takes 131 us, because the write-out of a job with two accumulators is not hidden.  A thread block per 128 x 256 tile, two on an SM: 140 us.
+constexpr int kScoreRows = 128, kScoreCols = 256, kScoreMaxStages = 8;
 constexpr int kScoreStageBytes = kScoreRows * 128;
-constexpr int kScoreMeans = kScoreStages * kScoreStageBytes;                 // offset of the means: two tiles of 256 rows x 128 bytes
-constexpr int kScoreBars = kScoreMeans + 2 * kScoreCols * 128;
-constexpr int kScoreSmem = kScoreBars + 128;
-constexpr int kScoreThreads = 192;  // warps 0-3 read the accumulator back, warp 4 loads, warp 5 multiplies
+constexpr int kScoreMeansBytes = 2 * kScoreCols * 128;                       // 256 rows of up to 128 dims
+constexpr int kScoreOut = 2 * kScoreMeansBytes + 4 * kScoreStageBytes;       // behind 4 stages and two tiles of means, or 8 and one: 32 x 32 floats per writing warp
+constexpr int kScoreBars = kScoreOut + 8 * 32 * 32 * 4;
+constexpr int kScoreSmem = kScoreBars + 208;
+constexpr int kScoreThreads = 320;  // warps 0-7 write (four an accumulator), warp 8 loads, warp 9 multiplies
 
-template <class T> __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap m_map, ScoresArgs a)
+// Job i of all: which sequence and head of keys, which queries, which tiles of means.
+struct ScoreJob {
+    uint32_t z, t, n, width;
+    __device__ ScoreJob(uint32_t i, uint32_t across, uint32_t down)
+    {
+        const uint32_t pairs = (across + 1) / 2;
+        z = i / (pairs * down);
+        n = i % (pairs * down) / down * 2;
+        t = i % down;
+        width = min(2u, across - n);
+    }
+};
+
+template <class T> __global__ void __launch_bounds__(kScoreThreads, 1) block_scores_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap m_map, ScoresArgs a, uint32_t jobs)
 {
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kScoreBars), *empty = full + kScoreStages, *means_in = empty + kScoreStages, *done = means_in + 1;
-    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(done + 1);  // [0] tensor memory, [1] gave up
-    const uint32_t n0 = blockIdx.x * kScoreCols, t0 = blockIdx.y * kScoreRows;
-    const uint32_t b = blockIdx.z / a.kv_heads, kv = blockIdx.z % a.kv_heads, group = a.heads / a.kv_heads;
-    const uint32_t halves = (a.dim + 63) / 64, steps = group * halves;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kScoreBars), *empty = full + kScoreMaxStages, *means_in = empty + kScoreMaxStages, *summed = means_in + 2, *written = summed + 2;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(written + 2);  // [0] tensor memory, [1] gave up
+    const uint32_t across = (a.blocks + kScoreCols - 1) / kScoreCols, down = (a.queries + kScoreRows - 1) / kScoreRows;
+    const uint32_t stages = across == 1 ? 8u : 4u, means_at = stages * kScoreStageBytes;
+    const uint32_t begin = (uint32_t)((uint64_t)jobs * blockIdx.x / gridDim.x), end = (uint32_t)((uint64_t)jobs * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t group = a.heads / a.kv_heads, halves = (a.dim + 63) / 64, steps = group * halves;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kScoreStages; ++s) {
+        for (int s = 0; s < kScoreMaxStages; ++s) {
             ptx::mbar_init(&full[s], 1);
             ptx::mbar_init(&empty[s], 1);
         }
-        ptx::mbar_init(means_in, 1);
-        ptx::mbar_init(done, 1);
+        for (int s = 0; s < 2; ++s) {
+            ptx::mbar_init(&means_in[s], 1);
+            ptx::mbar_init(&summed[s], 1);
+            ptx::mbar_init(&written[s], 4);
+        }
         misc[1] = 0;
         ptx::fence_mbar_init();
     }
-    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), kScoreCols);
+    if (warp == 0) tc::alloc(const_cast<uint32_t *>(&misc[0]), 2 * kScoreCols);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = misc[0];
     ptx::grid_wait();
     ptx::grid_release();
-    if (warp == 4 && lane == 0) {
-        ptx::mbar_expect_tx(means_in, halves * kScoreCols * 128);
-        for (uint32_t h = 0; h < halves; ++h) tc::tma_load4(smem + kScoreMeans + h * kScoreCols * 128, &m_map, (int)(h * 64), (int)kv, (int)n0, (int)b, means_in);
-        for (uint32_t i = 0; i < steps; ++i) {
-            const uint32_t s = i % kScoreStages;
-            if (!ptx::mbar_wait(&empty[s], ((i / kScoreStages) & 1u) ^ 1u)) {
-                misc[1] = 1;
-                break;
+    bool ok = true;
+    if (warp == 8) {
+        if (lane == 0) {
+            uint32_t k = 0, loads = 0, holds = ~0u;  // tiles of q so far; the means that are there: (z, n)
+            for (uint32_t i = begin; i < end && ok; ++i) {
+                const ScoreJob x(i, across, down);
+                const uint32_t b = x.z / a.kv_heads, kv = x.z % a.kv_heads;
+                if (holds != x.z * across + x.n) {
+                    holds = x.z * across + x.n;
+                    for (uint32_t j = k > stages ? k - stages : 0; j < k && ok; ++j) ok = ptx::mbar_wait(&empty[j % stages], (j / stages) & 1u);  // nothing reads the old ones any more
+                    if (!ok) break;
+                    for (uint32_t m = 0; m < x.width; ++m) {
+                        ptx::mbar_expect_tx(&means_in[m], halves * kScoreCols * 128);
+                        for (uint32_t h = 0; h < halves; ++h)
+                            tc::tma_load4(smem + means_at + m * kScoreMeansBytes + h * kScoreCols * 128, &m_map, (int)(h * 64), (int)kv, (int)((x.n + m) * kScoreCols), (int)b, &means_in[m]);
+                        loads += m ? 1u << 16 : 1u;
+                    }
+                }
+                for (uint32_t j = 0; j < steps; ++j, ++k) {
+                    const uint32_t s = k % stages;
+                    if (!(ok = ptx::mbar_wait(&empty[s], ((k / stages) & 1u) ^ 1u))) break;
+                    ptx::mbar_expect_tx(&full[s], kScoreStageBytes);
+                    tc::tma_load4(smem + s * kScoreStageBytes, &q_map, (int)(j % halves * 64), (int)(kv * group + j / halves), (int)(x.t * kScoreRows), (int)b, &full[s]);
+                }
             }
-            ptx::mbar_expect_tx(&full[s], kScoreStageBytes);
-            tc::tma_load4(smem + s * kScoreStageBytes, &q_map, (int)(i % halves * 64), (int)(kv * group + i / halves), (int)t0, (int)b, &full[s]);
+            if (!ok) {
+                misc[1] = 1;
+                // no copy stays in flight
+                if (loads & 0xffffu) ptx::mbar_wait(&means_in[0], (loads - 1) & 1u);
+                if (loads >> 16) ptx::mbar_wait(&means_in[1], ((loads >> 16) - 1) & 1u);
+                for (uint32_t j = k > stages ? k - stages : 0; j < k; ++j) ptx::mbar_wait(&full[j % stages], (j / stages) & 1u);
+            }
         }
-    } else if (warp == 5 && lane == 0) {
-        constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, kScoreRows, kScoreCols);
-        bool ok = ptx::mbar_wait(means_in, 0);
-        for (uint32_t i = 0; i < steps && ok; ++i) {
-            const uint32_t s = i % kScoreStages;
-            if (!(ok = ptx::mbar_wait(&full[s], (i / kScoreStages) & 1u))) break;
-            tc::fence_after();
-            const uint64_t ad = tc::desc_k(ptx::smem_u32(smem + s * kScoreStageBytes)), bd = tc::desc_k(ptx::smem_u32(smem + kScoreMeans + i % halves * kScoreCols * 128));
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t id = tc::idesc(std::is_same<T, __nv_bfloat16>::value, kScoreRows, kScoreCols);
+            const uint64_t q_k = tc::desc_k(ptx::smem_u32(smem)), m_k = tc::desc_k(ptx::smem_u32(smem) + means_at);
+            uint32_t k = 0, holds = ~0u, loads[2] = {0, 0}, uses[2] = {0, 0};
+            for (uint32_t i = begin; i < end && ok; ++i) {
+                const ScoreJob x(i, across, down);
+                const uint32_t first = x.width == 2 ? 0u : (i - begin) & 1u, last = x.width == 2 ? 1u : first;  // accumulators of the job
+                if (holds != x.z * across + x.n) {
+                    holds = x.z * across + x.n;
+                    for (uint32_t m = 0; m < x.width && ok; ++m) ok = ptx::mbar_wait(&means_in[m], loads[m]++ & 1u);
+                }
+                for (uint32_t c = first; c <= last && ok; ++c) ok = ptx::mbar_wait(&written[c], (uses[c]++ & 1u) ^ 1u);
+                if (!ok) break;
+                for (uint32_t j = 0; j < steps; ++j, ++k) {
+                    const uint32_t s = k % stages;
+                    if (!(ok = ptx::mbar_wait(&full[s], (k / stages) & 1u))) break;
+                    tc::fence_after();
+                    const uint64_t ad = q_k + s * (kScoreStageBytes >> 4);
+                    for (uint32_t c = first; c <= last; ++c) {
+                        const uint64_t bd = m_k + ((c - first) * (kScoreMeansBytes >> 4) + j % halves * (kScoreCols * 128 >> 4));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc::mma(tmem, ad + 2 * k, bd + 2 * k, id, i || k);
-            tc::commit(&empty[s]);
+                        for (int d = 0; d < 4; ++d) tc::mma(tmem + c * kScoreCols, ad + 2 * d, bd + 2 * d, id, j || d);
+                    }
+                    tc::commit(&empty[s]);
+                }
+                for (uint32_t c = first; c <= last; ++c) tc::commit(&summed[c]);
+            }
+            if (!ok) misc[1] = 1;
         }
-        if (!ok) misc[1] = 1;
-        tc::commit(done);
-    } else if (warp < 4) {
-        // accumulator -> rows of scores, 32 x 32 at a time through shared memory (the ring is free by then), so that a store is 128
-        // contiguous bytes of one row whatever the row's alignment
-        if (ptx::mbar_wait_warp(done, 0)) {
+    } else {
+        // accumulator -> rows of scores, 32 x 32 at a time through shared memory, so that a store is whole 128-byte pieces of rows: 16 bytes a
+        // lane where rows allow that, 4 otherwise (a loop that stored what it had just read took 17000 cycles a job, as long as the products)
+        unsigned char *part = smem + kScoreOut + warp * 32 * 128;
+        auto piece = [&](uint32_t row, uint32_t p) { return part + row * 128 + ((p ^ (row & 7)) << 4); };
+        const bool wide = a.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(a.scores) % 16 == 0;
+        const uint32_t acc = warp >> 2;
+        uint32_t uses = 0;
+        for (uint32_t i = begin; i < end; ++i) {
+            const ScoreJob x(i, across, down);
+            if (x.width == 1 && ((i - begin) & 1u) != acc) continue;
+            const uint32_t t0 = x.t * kScoreRows + (warp & 3) * 32, n0 = (x.n + (x.width == 2 ? acc : 0u)) * kScoreCols;
+            if (!(ok = ptx::mbar_wait_warp(&summed[acc], uses++ & 1u))) break;
             tc::fence_after();
-            float *tile = reinterpret_cast<float *>(smem) + warp * 32 * 33;
-            float *out = a.scores + (((uint64_t)b * a.kv_heads + kv) * a.queries + t0 + warp * 32) * a.blocks + n0;
-            const uint32_t rows = t0 + warp * 32 < a.queries ? min(32u, a.queries - t0 - warp * 32) : 0u;
+            float *out = a.scores + ((uint64_t)x.z * a.queries + t0) * a.blocks + n0;
+            const uint32_t rows = t0 < a.queries ? min(32u, a.queries - t0) : 0u;
             for (uint32_t c = 0; c < kScoreCols && n0 + c < a.blocks; c += 32) {
                 uint32_t v[32];
-                tc::ld32(tmem + ((warp * 32) << 16) + c, v);
+                tc::ld32(tmem + (((warp & 3) * 32) << 16) + acc * kScoreCols + c, v);
                 tc::wait_ld();
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = __uint_as_float(v[j]);
+                for (int p = 0; p < 8; ++p) *reinterpret_cast<uint4 *>(piece(lane, p)) = make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
                 __syncwarp();
-                if (n0 + c + lane < a.blocks)
-                    for (uint32_t r = 0; r < rows; ++r) __stcs(out + (uint64_t)r * a.blocks + c + lane, tile[r * 33 + lane]);
+                if (wide) {
+                    const uint32_t p = lane & 7, col = c + 4 * p;
+                    uint4 y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = *reinterpret_cast<const uint4 *>(piece(4 * k + lane / 8, p));
+                    if (n0 + col < a.blocks) {
+                        float *to = out + (uint64_t)(lane / 8) * a.blocks + col;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (4 * k + lane / 8 < rows) __stcs(reinterpret_cast<uint4 *>(to + (uint64_t)(4 * k) * a.blocks), y[k]);
+                    }
+                } else if (n0 + c + lane < a.blocks) {
+                    float *to = out + c + lane;
+#pragma unroll
+                    for (uint32_t r = 0; r < 32; r += 16) {
+                        float y[16];
+#pragma unroll
+                        for (uint32_t k = 0; k < 16; ++k) y[k] = *reinterpret_cast<const float *>(piece(r + k, lane >> 2) + (lane & 3) * 4);
+#pragma unroll
+                        for (uint32_t k = 0; k < 16; ++k)
+                            if (r + k < rows) __stcs(to + (uint64_t)(r + k) * a.blocks, y[k]);
+                    }
+                }
             }
-        } else if (lane == 0)
-            misc[1] = 1;
-        tc::fence_before();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&written[acc]);
+        }
+        if (!ok) misc[1] = 1;
     }
+    tc::fence_before();
     __syncthreads();
-    if (misc[1] && threadIdx.x == 0) {  // a wait gave up: report, and leave no copy in flight behind
-        atomicExch(&g_status, 1u);
-        ptx::mbar_wait(means_in, 0);
-        for (uint32_t s = 0; s < kScoreStages; ++s)
-            for (uint32_t p = 0; p < 2; ++p) ptx::mbar_wait(&full[s], p);
-    }
+    if (threadIdx.x == 0 && misc[1]) atomicExch(&g_status, 1u);
     if (warp == 0) {
         tc::fence_after();
-        tc::dealloc(tmem, kScoreCols);
+        tc::dealloc(tmem, 2 * kScoreCols);
     }
 }
 
@@ -321,7 +405,6 @@ cudaError_t launch_block_means(const MeansArgs &a, cudaStream_t s)
 
 cudaError_t launch_block_scores(const ScoresArgs &a, int sm_count, cudaStream_t s)
 {
-    (void)sm_count;
     if (!a.batch || !a.queries || !a.kv_heads || !a.blocks) return cudaSuccess;
     const bool bf16 = a.dtype == CUTESPMM_BF16;
     CUtensorMap q_map, m_map;
@@ -329,9 +412,11 @@ cudaError_t launch_block_scores(const ScoresArgs &a, int sm_count, cudaStream_t 
     if (e == cudaSuccess) e = tc::make_map(&m_map, bf16, a.means, a.dim, a.kv_heads, a.blocks, a.batch, a.m_head, a.m_block, a.m_batch, kScoreCols);
     if (e == cudaSuccess) e = bf16 ? allow_dynamic_smem<block_scores_kernel<__nv_bfloat16>>(kScoreSmem) : allow_dynamic_smem<block_scores_kernel<__half>>(kScoreSmem);
     if (e != cudaSuccess) return e;
-    const dim3 grid((a.blocks + kScoreCols - 1) / kScoreCols, (a.queries + kScoreRows - 1) / kScoreRows, a.batch * a.kv_heads);
-    return bf16 ? launch_overlapped(block_scores_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a)
-                : launch_overlapped(block_scores_kernel<__half>, grid, dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a);
+    const uint64_t jobs = (uint64_t)((a.blocks + 2 * kScoreCols - 1) / (2 * kScoreCols)) * ((a.queries + kScoreRows - 1) / kScoreRows) * a.batch * a.kv_heads;
+    if (jobs >> 31) return cudaErrorInvalidConfiguration;
+    const unsigned grid = (unsigned)(jobs < (uint64_t)sm_count ? jobs : (uint64_t)sm_count);
+    return bf16 ? launch_overlapped(block_scores_kernel<__nv_bfloat16>, dim3(grid), dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a, (uint32_t)jobs)
+                : launch_overlapped(block_scores_kernel<__half>, dim3(grid), dim3(kScoreThreads), kScoreSmem, s, q_map, m_map, a, (uint32_t)jobs);
 }
 
 cudaError_t launch_select_blocks(const SelectArgs &a, int sm_count, cudaStream_t s)

@@ -173,7 +173,7 @@ def test_block_means(dtype, batch, keys, kv, dim, block):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("batch,queries,kv,group,dim,blocks", [(1, 1, 1, 1, 64, 1), (2, 129, 2, 3, 72, 33), (1, 300, 1, 8, 128, 257), (3, 64, 4, 2, 8, 100), (1, 40, 2, 16, 80, 600)])
+@pytest.mark.parametrize("batch,queries,kv,group,dim,blocks", [(1, 1, 1, 1, 64, 1), (2, 129, 2, 3, 72, 33), (1, 300, 1, 8, 128, 257), (3, 64, 4, 2, 8, 100), (1, 40, 2, 16, 80, 600), (2, 1400, 3, 1, 64, 1300), (7, 260, 3, 2, 128, 530)])
 def test_block_scores(dtype, batch, queries, kv, group, dim, blocks):
     torch.manual_seed(queries)
     q = torch.randn(batch, queries, kv * group, dim, device="cuda").to(dtype)
