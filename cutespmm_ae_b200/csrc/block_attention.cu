@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 // spent a third of a tile's time between them.
 // Rows whose query does not name a tile have P = 0 there.  Multiplying only what is named, on mma.sync with a query's eight heads as the columns of
 // an instruction, was slower for every group, block size and dim tried with the blocks of a selection: 8192 queries, 32 heads, 16 blocks of 64, where
-// 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 510; 4096 queries, one head to a group, 16 blocks of 16 302 against 226.
+// 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 407 now; 4096 queries, one head to a group, 16 blocks of 16 302 against 94.
 // The maximum is raised only when a score exceeds it by 2^8, so that O is rescaled in tensor memory a few times per row instead of once per
 // tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM: one multiplies while the other's rows are at work.
 // 0 times a value that is no number is not 0: rows of V behind the last visible key are zeroed as they land, and a row whose result is

@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     }
 }
 
-// Key tiles that no query names are zero; the partial sums of those with several work items are added in order.
+// Key tiles that no query names are zero; the partial sums of those with several work items are added in order.  Eight blocks of threads a tile.
 template <class T, int DP> __global__ void __launch_bounds__(256) dkv_join_kernel(TurnArgs p)
 {
     ptx::grid_wait();
@@ -784,7 +784,7 @@ template <class T, int DP> __global__ void __launch_bounds__(256) dkv_join_kerne
     const uint32_t tile = row % p.tiles, bh = row / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
     const uint32_t n = min(kKeyTile, a.keys - tile * kKeyTile);
     const float *src = p.partial + (uint64_t)p.first_slot[row] * 2 * kKeyTile * DP;
-    for (uint32_t i = threadIdx.x; i < 2 * n * (DP / 4); i += 256) {
+    for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < 2 * n * (DP / 4); i += 256 * gridDim.y) {
         const uint32_t d = i % (DP / 4) * 4, key = i / (DP / 4) % n, is_dk = i / (DP / 4) / n;
         if (d >= a.dim) continue;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -851,7 +851,7 @@ template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count
     if ((e = allow_dynamic_smem<block_attention_dkv_kernel<T, DP>>(DkvSmem<DP>::kBytes)) != cudaSuccess) return e;
     const uint64_t blocks = l.max_items < (uint64_t)sm_count ? l.max_items : (uint64_t)sm_count;
     if ((e = launch_overlapped(block_attention_dkv_kernel<T, DP>, dim3((unsigned)blocks), dim3(kDkvThreads), DkvSmem<DP>::kBytes, s, k_map, v_map, p)) != cudaSuccess) return e;
-    return launch_overlapped(dkv_join_kernel<T, DP>, dim3((unsigned)l.tile_rows), dim3(256), 0, s, p);
+    return launch_overlapped(dkv_join_kernel<T, DP>, dim3((unsigned)l.tile_rows, 8), dim3(256), 0, s, p);
 }
 
 }  // namespace

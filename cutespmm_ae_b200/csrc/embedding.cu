@@ -124,15 +124,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs a)
     // per digit: keys of all blocks, and of the blocks in front of this one; two digits a thread
     static_assert(kMaxBins == 2 * kSortThreads, "two digits per thread");
     uint32_t before[2] = {0, 0}, all[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t b = 2 * threadIdx.x + h;
-        if (b >= a.bins) continue;
-#pragma unroll 8
+    if (2 * threadIdx.x < a.bins) {
+#pragma unroll 16
         for (uint32_t k = 0; k < gridDim.x; ++k) {
-            const uint32_t c = a.counts[(uint64_t)k * a.bins + b];
-            all[h] += c;
-            if (k < blockIdx.x) before[h] += c;
+            const uint2 c = *reinterpret_cast<const uint2 *>(a.counts + (uint64_t)k * a.bins + 2 * threadIdx.x);  // at least two bins: a pass has a bit or more
+            all[0] += c.x;
+            all[1] += c.y;
+            before[0] += k < blockIdx.x ? c.x : 0u;
+            before[1] += k < blockIdx.x ? c.y : 0u;
         }
     }
     // keys of smaller digits: a scan over the threads

@@ -354,6 +354,15 @@ def test_attention_and_its_gradients(dtype, form):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv,group,dim,block,count", [(1, 1, 8, 16, 128), (1, 2, 128, 32, 100), (2, 8, 64, 16, 60)])
+def test_many_blocks_of_a_long_cache(kv, group, dim, block, count):
+    """Queries whose blocks lie all over a cache of 150000 keys: tiles of queries get smaller where their lists would not fit."""
+    torch.manual_seed(group)
+    q, k, v = attention_inputs(torch.bfloat16, 1, 130, 150000, kv, group, dim)
+    check_attention(q, k, v, random_blocks(1, kv, 130, count, 150000, block, share=0.1), block, grad=group < 8)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("form", [(2, 65, 300, 2, 8, 128, 64, 4), (2, 65, 300, 2, 1, 64, 16, 8), (3, 40, 100, 1, 4, 64, 32, 3), (2, 50, 256, 1, 2, 128, 128, 2)])
 def test_rows_that_see_nothing_and_keys_that_nobody_sees(dtype, form):
@@ -371,7 +380,9 @@ def test_rows_that_see_nothing_and_keys_that_nobody_sees(dtype, form):
         v[b, top[b] :] = math.inf
     blocks = random_blocks(batch, kv, queries, count, keys, block)
     blocks[0, :, 5] = -1
-    got = check_attention(q, k, v, blocks, block, visible)
+    dout = torch.randn(q.shape, device="cuda").to(dtype)
+    dout[visible <= 0] = math.nan  # padded positions: nothing of them reaches a gradient
+    got = check_attention(q, k, v, blocks, block, visible, dout=dout)
     assert not got[0][visible <= 0].any() and not got[1][visible <= 0].any()
     assert not got[0][0, 5].any()
     # a key that later queries see may hold anything as far as earlier ones are concerned, and so may a block that others name
