@@ -131,10 +131,12 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, 
 // Rows whose query does not name a tile have P = 0 there.  Multiplying only what is named, on mma.sync with a query's eight heads as the columns of
 // an instruction, was slower for every group, block size and dim tried with the blocks of a selection: 8192 queries, 32 heads, 16 blocks of 64, where
 // 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 407 now; 4096 queries, one head to a group, 16 blocks of 16 302 against 94.
-// The maximum is raised only when a score exceeds it by 2^8, so that O is rescaled in tensor memory a few times per row instead of once per
+// The maximum is raised only when a score exceeds it by 8 (of the base-2 exponent), so that O is rescaled in tensor memory a few times per row instead of once per
 // tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM: one multiplies while the other's rows are at work.
 // 0 times a value that is no number is not 0: rows of V behind the last visible key are zeroed as they land, and a row whose result is
 // not finite is formed again, key by key, from what its query looks at (exact_row).
+// Measured, forward alone: 8192 queries, 32 heads of dim 128 over 4 heads of keys, 16 blocks of 64: 354 to 410 us (tensor pipe 45 % busy, issue slots 36 %);
+// 16384 queries, 16 heads over 2, 32 blocks: 717 us.  Bound: a row's way from S to P (1100 cycles a tile, half of it exponentials), twice on an SM.
 constexpr int kTcThreads = 224;
 constexpr int kTcStages = 2;  // of keys, of values, and of S in tensor memory
 constexpr uint32_t kTcO = 128, kTcCols = 256;  // columns of tensor memory: two buffers of S, O
@@ -396,7 +398,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
 // One query's heads of one head of keys: its blocks, in pieces of 16 keys, are dealt over the warps of a cluster of thread blocks.  A
 // warp fills a ring of its own (its lane 0 issues the loads) and keeps its own softmax state; the states are joined in the
 // order of the warps, first inside a thread block, then over the cluster through distributed shared memory: no scratch, no counters, one
-// launch.  Bound: HBM (the named blocks once) in batches, a chain of latencies for one sequence.
+// launch.  Bound: HBM (the named blocks once) in batches: 64 tokens, 64 heads over 8, 48 blocks of 64 keys of a paged cache 148 us, 5.4 TB/s (one thread block
+// an SM with rings twice as deep: 214 us).  A chain of latencies for one sequence: 8 us.
 constexpr int kSplitWarps = 4, kSplitUnit = 16;
 template <int DP> constexpr int kSplitStages = DP == 128 ? 2 : 4;  // 64 KB of keys and values: three thread blocks share an SM
 constexpr uint32_t kSplitCount = 128;  // most blocks of a query

@@ -28,7 +28,8 @@ __device__ uint32_t g_status;  // set to 1 (dq) or 2 (dk, dv) when a bounded wai
 // The forward kernel's 128 rows and union of key tiles.  Per tile S = Q K^T and D = dO V^T (128 x 64, two buffers of tensor memory), dS from
 // registers back into S's columns as 16-bit operand, dQ += dS K with the same bytes of K.  Q and dO stay in tensor memory for the whole kernel: an
 // operand A in shared memory would be read again for every 16 dims, 6 KB for 32 cycles of multiplying.  Eight warps form dS: a row's lse and
-// delta are one value each, two threads share a row.  Warp 8 loads, warp 9 issues S and D, warp 10 dQ.  A row whose dq is not finite is formed again from
+// delta are one value each, two threads share a row.  Warp 8 loads, warp 9 issues S and D, warp 10 dQ.  Measured: 8192 queries, 32 heads of dim 128 over 4,
+// 16 blocks of 64: 585 us (q and dout in shared memory, one issuing warp: 713), tensor pipe 39 % busy; bound by the round trip of a tile through its two buffers.  A row whose dq is not finite is formed again from
 // what its query looks at.
 constexpr int kDqWarps = 8, kDqThreads = (kDqWarps + 3) * 32, kDqStages = 4;
 constexpr uint32_t kDqBuffer = 128, kDqSum = 256, kDqQ = 384, kDqDo = 448, kDqCols = 512;
@@ -442,6 +443,9 @@ __global__ void __launch_bounds__(1024) pattern_items_kernel(TurnArgs p)
 // with the same shared-memory bytes of Q and dO serving as row-major operand of the first pair and as transposed operand of the second.
 // The tile after is multiplied while this one's P and dS are formed.  Every query names its keys by choice, so no row of a tile is
 // wasted, however little neighbouring queries agree; this is what makes the 128-row instruction the right one here.
+// Measured: 8192 queries, 32 heads of dim 128 over 4, 16 blocks of 64: 505 us, 3800 cycles a tile, of which the products take 2000: 62 each for 32 of
+// arithmetic, because both operands come from shared memory (6 KB at 128 bytes a cycle).  Bound: a stage's round trip (gather 2200 cycles, S and D 1000, P and dS 1100, sums
+// 1000) over the two stages that shared memory holds.
 constexpr int kDkvWarps = 8, kDkvLoaders = 8;  // warps 0-7 form P and dS, 8-15 load, warp 16 multiplies
 constexpr int kDkvThreads = (kDkvWarps + kDkvLoaders + 1) * 32;
 constexpr int kDkvStages = 2;
