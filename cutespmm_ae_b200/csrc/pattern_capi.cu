@@ -26,9 +26,13 @@ bool aligned(const void *p, const int64_t *strides)
         if (strides[i] < 0 || strides[i] % 8 || strides[i] >= (int64_t)1 << 39) return false;
     return true;
 }
+// Kernels load and store 16 bytes at a time in results as well; every other array has to lie on its elements' own grid.
+bool on_grid(const void *p, uint32_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+uint32_t bytes_of(int dtype) { return dtype == CUTESPMM_F32 ? 4 : 2; }
+const char *const kOffElements = "a pointer is not aligned to its elements";
 bool fits_grid(uint64_t n) { return n <= 65535; }
 
-int check_embedding(int dtype, uint64_t vocab, uint32_t dim, uint64_t ld_a, uint64_t ld_b, const void *tokens, int token_bytes, uint64_t count)
+int check_embedding(int dtype, uint64_t vocab, uint32_t dim, const void *a, uint64_t ld_a, const void *b, uint64_t ld_b, const void *tokens, int token_bytes, uint64_t count)
 {
     if (dtype != CUTESPMM_F32 && dtype != CUTESPMM_F16 && dtype != CUTESPMM_BF16) return refuse(CUTESPMM_EINVAL, "dtype must be CUTESPMM_F32, CUTESPMM_F16 or CUTESPMM_BF16");
     if (token_bytes != 4 && token_bytes != 8) return refuse(CUTESPMM_EINVAL, "tokens must be int32 or int64 (token_bytes 4 or 8)");
@@ -36,6 +40,7 @@ int check_embedding(int dtype, uint64_t vocab, uint32_t dim, uint64_t ld_a, uint
     if (vocab >> 31 || count >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "more than 2^31 - 1 rows or tokens");
     if (dim >> 30) return refuse(CUTESPMM_EUNSUPPORTED, "dim must be below 2^30");
     if (count && !tokens) return refuse(CUTESPMM_EINVAL, "tokens is NULL");
+    if (!on_grid(a, bytes_of(dtype)) || !on_grid(b, bytes_of(dtype)) || !on_grid(tokens, (uint32_t)token_bytes)) return refuse(CUTESPMM_EINVAL, kOffElements);
     return CUTESPMM_OK;
 }
 
@@ -74,6 +79,7 @@ int to_args(const cutespmm_block_attention_t *d, AttentionArgs &a)
     if (work && d->count && !d->blocks) return refuse(CUTESPMM_EINVAL, "blocks is NULL");
     if (!aligned(d->q, d->q_strides) || !aligned(d->k, d->k_strides) || !aligned(d->v, d->v_strides))
         return refuse(CUTESPMM_EINVAL, "q, k and v must be 16-byte aligned, their strides multiples of 8 elements");
+    if (!on_grid(d->blocks, 4) || !on_grid(d->visible, 4) || !on_grid(d->pages, 4)) return refuse(CUTESPMM_EINVAL, kOffElements);
     a = AttentionArgs{};
     a.dtype = (int)d->dtype;
     a.q = d->q; a.k = d->k; a.v = d->v;
@@ -95,7 +101,7 @@ extern "C" {
 int cutespmm_embedding(int dtype, const void *table_dev, uint64_t ld_table, uint64_t vocab, uint32_t dim, const void *tokens_dev, int token_bytes, uint64_t count, float scale,
                        void *out_dev, uint64_t ld_out, void *stream)
 {
-    int st = check_embedding(dtype, vocab, dim, ld_table, ld_out, tokens_dev, token_bytes, count);
+    int st = check_embedding(dtype, vocab, dim, table_dev, ld_table, out_dev, ld_out, tokens_dev, token_bytes, count);
     if (st != CUTESPMM_OK) return st;
     if (count && dim && ((vocab && !table_dev) || !out_dev)) return refuse(CUTESPMM_EINVAL, "table or out is NULL");
     int dev = -1, sms = 0;
@@ -110,7 +116,7 @@ uint64_t cutespmm_embedding_grad_workspace(uint64_t count, uint64_t vocab, uint3
 int cutespmm_embedding_grad(int dtype, const void *dout_dev, uint64_t ld_dout, const void *tokens_dev, int token_bytes, uint64_t count, uint64_t vocab, uint32_t dim, float scale,
                             void *dtable_dev, uint64_t ld_dtable, void *workspace_dev, uint64_t workspace_bytes, void *stream)
 {
-    int st = check_embedding(dtype, vocab, dim, ld_dout, ld_dtable, tokens_dev, token_bytes, count);
+    int st = check_embedding(dtype, vocab, dim, dout_dev, ld_dout, dtable_dev, ld_dtable, tokens_dev, token_bytes, count);
     if (st != CUTESPMM_OK) return st;
     if (vocab == 0 || dim == 0) return CUTESPMM_OK;
     if ((count && !dout_dev) || !dtable_dev) return refuse(CUTESPMM_EINVAL, "dout or dtable is NULL");
@@ -133,6 +139,7 @@ int cutespmm_block_means(int dtype, const void *k_dev, const int64_t k_strides[3
     if (!fits_grid(blocks)) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65535 blocks of keys");
     if (!k_strides || !aligned(k_dev, k_strides)) return refuse(CUTESPMM_EINVAL, "k must be 16-byte aligned, its strides multiples of 8 elements");
     if (batch && blocks && (!k_dev || !means_dev)) return refuse(CUTESPMM_EINVAL, "k or means is NULL");
+    if (!on_grid(lengths_dev, 4) || !on_grid(means_dev, 2)) return refuse(CUTESPMM_EINVAL, kOffElements);
     int dev = -1, sms = 0;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
     NvtxRange range("cutespmm: block means");
@@ -150,6 +157,7 @@ int cutespmm_block_scores(int dtype, const void *q_dev, const int64_t q_strides[
     if (blocks > 65536) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65536 blocks of keys");
     if (((uint64_t)(blocks + 255) / 256 * ((queries + 127) / 128) * batch * kv_heads) >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "too many queries and blocks for one call");
     if (batch && queries && heads && blocks && (!q_dev || !means_dev || !scores_dev)) return refuse(CUTESPMM_EINVAL, "q, means or scores is NULL");
+    if (!on_grid(scores_dev, 4)) return refuse(CUTESPMM_EINVAL, kOffElements);
     int dev = -1, sms = 0;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
     NvtxRange range("cutespmm: block scores");
@@ -168,6 +176,7 @@ int cutespmm_select_blocks(const float *scores_dev, const int64_t s_strides[3], 
     if (keys >> 28 || queries >> 28 || count >> 16) return refuse(CUTESPMM_EUNSUPPORTED, "too many keys, queries or blocks per query");
     if (!fits_grid((uint64_t)batch * kv_heads)) return refuse(CUTESPMM_EUNSUPPORTED, "batch * kv_heads must be at most 65535");
     if (batch && kv_heads && queries && count && ((blocks && (!scores_dev || !s_strides)) || !blocks_dev)) return refuse(CUTESPMM_EINVAL, "scores, strides or blocks is NULL");
+    if (!on_grid(scores_dev, 4) || !on_grid(visible_dev, 4) || !on_grid(blocks_dev, 4)) return refuse(CUTESPMM_EINVAL, kOffElements);
     int dev = -1, sms = 0, st;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
     NvtxRange range("cutespmm: block selection");
@@ -186,6 +195,7 @@ int cutespmm_block_attention(const cutespmm_block_attention_t *args, void *out_d
     int st = to_args(args, a);
     if (st != CUTESPMM_OK) return st;
     if (a.batch && a.queries && a.heads && (!out_dev || !lse_dev)) return refuse(CUTESPMM_EINVAL, "out or lse is NULL");
+    if (!on_grid(out_dev, 16) || !on_grid(lse_dev, 4)) return refuse(CUTESPMM_EINVAL, "out must be 16-byte aligned, lse aligned to its elements");
     int dev = -1, sms = 0;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
     NvtxRange range("cutespmm: block attention");
@@ -210,6 +220,8 @@ int cutespmm_block_attention_grad(const cutespmm_block_attention_t *args, const 
     if (!dout_strides || !aligned(dout_dev, dout_strides)) return refuse(CUTESPMM_EINVAL, "dout must be 16-byte aligned, its strides multiples of 8 elements");
     if (a.batch && a.queries && a.heads && (!dout_dev || !out_dev || !lse_dev || !dq_dev)) return refuse(CUTESPMM_EINVAL, "dout, out, lse or dq is NULL");
     if (a.batch && a.keys && (!dk_dev || !dv_dev)) return refuse(CUTESPMM_EINVAL, "dk or dv is NULL");
+    if (!on_grid(out_dev, 16) || !on_grid(dq_dev, 16) || !on_grid(dk_dev, 16) || !on_grid(dv_dev, 16) || !on_grid(lse_dev, 4))
+        return refuse(CUTESPMM_EINVAL, "out, dq, dk and dv must be 16-byte aligned, lse aligned to its elements");
     const uint64_t need = block_attention_grad_workspace(a);
     if (need && (!workspace_dev || reinterpret_cast<uintptr_t>(workspace_dev) % 256 || workspace_bytes < need))
         return refuse(CUTESPMM_EINVAL, "workspace must be 256-byte aligned and hold cutespmm_block_attention_grad_workspace() bytes");

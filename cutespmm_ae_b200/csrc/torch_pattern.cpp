@@ -240,7 +240,9 @@ std::tuple<Tensor, Tensor, Tensor> op_block_attention_grad(const Tensor &dout, c
     TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.sizes() == at::IntArrayRef({q.size(0), q.size(2), q.size(1)}), "lse must be a float32 tensor [batch, heads, queries]");
     want_cuda(q, {dout, out, lse});
     const Operand g(dout);
-    const Tensor o = out.contiguous(), l = lse.contiguous();
+    Tensor o = out.contiguous();
+    if (o.numel() && reinterpret_cast<uintptr_t>(o.const_data_ptr()) % 16) o = o.clone(at::MemoryFormat::Contiguous);  // a view off the 16-byte grid
+    const Tensor l = lse.contiguous();
     Tensor dq = empty_like_of(q.sizes(), q), dk = empty_like_of(k.sizes(), k), dv = empty_like_of(v.sizes(), v);
     if (!dq.numel()) return {dq, dk.zero_(), dv.zero_()};
     const Tensor work = scratch(cutespmm_block_attention_grad_workspace(&at.args), q);

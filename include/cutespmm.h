@@ -266,7 +266,8 @@ int cutespmm_spmm_csr_noalloc(uint32_t M, uint32_t K, uint32_t nnz, const uint32
  * plan, no state, no allocation (where a call needs scratch, the caller passes it).  Device pointers refer to the current CUDA
  * device, work is ordered on `stream`, nothing waits for the device; calls may overlap on any streams and be captured.
  *
- * Elements are fp32, fp16 or bf16; sums are held in fp32 and rounded once. */
+ * Elements are fp32, fp16 or bf16; sums are held in fp32 and rounded once.  Arrays are aligned to their elements, those of the attention
+ * to more (below); what is not is refused (CUTESPMM_EINVAL). */
 typedef enum { CUTESPMM_F32 = 0, CUTESPMM_F16 = 1, CUTESPMM_BF16 = 2 } cutespmm_dtype_t;
 
 /* out[i] = scale * table[tokens[i]] for i < count: rows of dim elements, leading dimensions in elements.  tokens: int32 or int64
@@ -285,7 +286,7 @@ int cutespmm_embedding_grad(int dtype, const void *dout_dev, uint64_t ld_dout, c
 /* Attention over selected blocks.  Keys are cut into blocks of `block` (16, 32, 64 or 128) consecutive ones; kv_heads heads of keys
  * and values serve `heads` = group * kv_heads query heads, head h using head h / group of the keys.  dim: a multiple of 8, at most
  * 128.  q, k, v and the means are fp16 or bf16.  Operands are [batch][row][head][dim] with strides in elements, dim contiguous,
- * strides multiples of 8 and pointers 16-byte aligned.
+ * strides multiples of 8 and pointers 16-byte aligned.  So are out, dq, dk and dv.
  *
  * visible[b][t]: how many keys query t of sequence b sees -- the first that many; 0: the query is padding and its output zero;
  * clamped to [0, keys].  NULL: causal, the last query sees every key (query t sees keys - queries + 1 + t). */

@@ -753,3 +753,66 @@ def test_fake_kernels_give_shapes():
         out, lse = torch.ops.cutespmm.block_attention(q, k, k, blocks, 16, None, 1.0, None)
         assert out.shape == q.shape and lse.shape == (2, 4, 5)
         assert [g.shape for g in torch.ops.cutespmm.block_attention_grad(out, q, k, k, out, lse, blocks, 16, None, 1.0)] == [q.shape, k.shape, k.shape]
+
+
+# ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
+
+
+def attention_call(q, k, v, blocks, block, queries, heads, *, batch=1, kv_heads=2, dim=64, keys=64, count=2, visible=None, pages=None, page_cols=0):
+    """The C ABI's description of a call (cutespmm_block_attention_t), operands contiguous."""
+    import ctypes as C
+
+    class Call(C.Structure):
+        _fields_ = [(n, C.c_uint32) for n in "struct_size dtype batch queries heads kv_heads dim keys block count".split()]
+        _fields_ += [(n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides")]
+        _fields_ += [(n, C.c_void_p) for n in ("blocks", "visible", "pages")] + [("page_cols", C.c_uint32), ("num_pages", C.c_uint32), ("scale", C.c_float)]
+
+    c = Call(C.sizeof(Call), 1, batch, queries, heads, kv_heads, dim, keys, block, count, q, k, v)
+    c.q_strides[:] = queries * heads * dim, heads * dim, dim
+    c.k_strides[:] = c.v_strides[:] = keys * kv_heads * dim, kv_heads * dim, dim
+    c.blocks, c.visible, c.pages, c.scale = blocks, visible, pages, 0.125
+    c.page_cols = c.num_pages = page_cols
+    return c
+
+
+def test_pointers_off_their_grid_are_refused():
+    """Kernels store and load 16 bytes at a time in out and the gradients; the rest lies on its elements' grid.  Checked before a device is asked."""
+    import ctypes as C
+
+    lib, p, EINVAL = cs.lib, 1 << 20, -1
+    s3 = (C.c_int64 * 3)(64, 64, 64)
+    call = C.byref(attention_call(p, p, p, p, 16, 4, 4))
+    assert lib.cutespmm_block_attention(call, p + 8, p, None) == EINVAL
+    assert lib.cutespmm_block_attention(call, p, p + 2, None) == EINVAL
+    need = lib.cutespmm_block_attention_grad_workspace(call)
+    assert need
+    for i in range(5):  # out, lse, dq, dk, dv
+        at = [p] * 5
+        at[i] += 2 if i == 1 else 8
+        assert lib.cutespmm_block_attention_grad(call, p, s3, at[0], at[1], at[2], at[3], at[4], p, need, None) == EINVAL
+    for bad in (dict(visible=p + 2), dict(pages=p + 1, page_cols=4), dict(blocks=p + 2)):
+        assert lib.cutespmm_block_attention(C.byref(attention_call(p, p, p, bad.pop("blocks", p), 16, 4, 4, **bad)), p, p, None) == EINVAL
+    for table, tokens, out in ((p + 1, p, p), (p, p + 2, p), (p, p, p + 1)):
+        assert lib.cutespmm_embedding(2, table, 8, 4, 8, tokens, 4, 2, 1.0, out, 8, None) == EINVAL
+        assert lib.cutespmm_embedding_grad(2, table, 8, tokens, 4, 2, 4, 8, 1.0, out, 8, p, 1 << 30, None) == EINVAL
+    assert lib.cutespmm_embedding(0, p + 2, 8, 4, 8, p, 4, 2, 1.0, p, 8, None) == EINVAL
+    assert lib.cutespmm_embedding(0, p, 8, 4, 8, p + 4, 8, 2, 1.0, p, 8, None) == EINVAL
+    assert lib.cutespmm_block_means(1, p, s3, p + 2, 1, 16, 1, 64, 16, p, None) == EINVAL
+    assert lib.cutespmm_block_means(1, p, s3, None, 1, 16, 1, 64, 16, p + 1, None) == EINVAL
+    assert lib.cutespmm_block_scores(1, p, s3, p, s3, 1, 2, 4, 2, 3, 64, p + 2, None) == EINVAL
+    for scores, visible, blocks in ((p + 2, p, p), (p, p + 1, p), (p, p, p + 2)):
+        assert lib.cutespmm_select_blocks(scores, s3, visible, 1, 1, 1, 4, 64, 16, 2, 1, 1, blocks, None) == EINVAL
+
+
+@pytest.mark.gpu
+def test_gradient_from_an_output_off_the_grid():
+    """`out` as a view that begins two bytes behind the 16-byte grid is copied; the gradients are the same."""
+    torch.manual_seed(22)
+    q, k, v = attention_inputs(torch.bfloat16, 1, 40, 40, 2, 2, 64)
+    blocks = random_blocks(1, 2, 40, 3, 40, 16)
+    out, lse = torch.ops.cutespmm.block_attention(q, k, v, blocks, 16, None, 0.125, None)
+    off = torch.cat([out.new_zeros(1), out.flatten()])[1:].view(out.shape)
+    assert off.data_ptr() % 16 == 2 and off.is_contiguous()
+    dout = torch.randn(q.shape, device="cuda").bfloat16()
+    for a, b in zip(torch.ops.cutespmm.block_attention_grad(dout, q, k, v, off, lse, blocks, 16, None, 0.125), torch.ops.cutespmm.block_attention_grad(dout, q, k, v, out, lse, blocks, 16, None, 0.125)):
+        assert torch.equal(a, b)
