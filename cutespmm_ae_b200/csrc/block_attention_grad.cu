@@ -860,16 +860,18 @@ template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count
 
 }  // namespace
 
-uint64_t block_attention_grad_workspace(const AttentionArgs &a) { return GradLayout(a).total; }
+// Whether some query may look at some key; without one there is no pattern to turn round, and sizes that the layout divides by are zero.
+static bool has_pairs(const AttentionArgs &a) { return a.batch && a.queries && a.heads && a.count; }
+
+uint64_t block_attention_grad_workspace(const AttentionArgs &a) { return has_pairs(a) ? GradLayout(a).total : 0; }
 
 cudaError_t launch_block_attention_grad(const AttentionArgs &a, int sm_count, cudaStream_t s)
 {
-    if (!a.batch || !a.heads || !a.dim) return cudaSuccess;
-    const uint64_t kv_bytes = (uint64_t)a.batch * a.keys * a.kv_heads * a.dim * 2;
-    if (!a.queries || !a.count) {  // nobody looks at any key
+    if (!has_pairs(a)) {  // nobody looks at any key
+        const uint64_t kv_bytes = (uint64_t)a.batch * a.keys * a.kv_heads * a.dim * 2, q_bytes = (uint64_t)a.batch * a.queries * a.heads * a.dim * 2;
         cudaError_t e = cudaSuccess;
         if (kv_bytes && (e = cudaMemsetAsync(a.dk, 0, kv_bytes, s)) == cudaSuccess) e = cudaMemsetAsync(a.dv, 0, kv_bytes, s);
-        if (e == cudaSuccess && a.queries) e = cudaMemsetAsync(a.dq, 0, (uint64_t)a.batch * a.queries * a.heads * a.dim * 2, s);
+        if (e == cudaSuccess && q_bytes) e = cudaMemsetAsync(a.dq, 0, q_bytes, s);
         return e;
     }
     if (a.dtype == CUTESPMM_BF16) return a.dim <= 64 ? launch_grad<__nv_bfloat16, 64>(a, sm_count, s) : launch_grad<__nv_bfloat16, 128>(a, sm_count, s);

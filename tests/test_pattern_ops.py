@@ -816,3 +816,45 @@ def test_gradient_from_an_output_off_the_grid():
     dout = torch.randn(q.shape, device="cuda").bfloat16()
     for a, b in zip(torch.ops.cutespmm.block_attention_grad(dout, q, k, v, off, lse, blocks, 16, None, 0.125), torch.ops.cutespmm.block_attention_grad(dout, q, k, v, out, lse, blocks, 16, None, 0.125)):
         assert torch.equal(a, b)
+
+
+EMPTY = [dict(queries=0), dict(heads=0), dict(batch=0), dict(count=0), dict(keys=0), dict(queries=0, keys=0)]
+
+
+def empty_call(empty, q=1 << 20, k=1 << 20, v=1 << 20, blocks=1 << 20):
+    sizes = dict(dict(queries=4, heads=4), **empty)
+    return attention_call(q, k, v, blocks, 16, sizes.pop("queries"), sizes.pop("heads"), **sizes)
+
+
+@pytest.mark.parametrize("empty", EMPTY)
+def test_workspace_of_an_empty_gradient(empty):
+    """In a process of its own: sizes of zero ended it."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+
+    code = ("import ctypes as C, test_pattern_ops as t; n = t.cs.lib.cutespmm_block_attention_grad_workspace(C.byref(t.empty_call(%r))); "
+            "print(n); assert (n > 0) == %r") % (empty, set(empty) == {"keys"})  # dq alone takes delta
+    res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env={**__import__("os").environ, "PYTHONPATH": f"{ROOT}:{ROOT / 'tests'}"}, capture_output=True, text=True)
+    assert res.returncode == 0, (res.returncode, res.stdout, res.stderr)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("empty", EMPTY)
+def test_empty_gradients_of_the_c_abi(empty):
+    """Without queries, heads or blocks nobody looks at any key: the gradients that have elements become zero."""
+    import ctypes as C
+
+    q, k, v, out = (torch.randn(4096, device="cuda").half() for _ in range(4))
+    blocks, lse = torch.zeros(64, device="cuda", dtype=torch.int32), torch.zeros(64, device="cuda")
+    grads = [torch.full((64 * 2 * 64 + 8,), 3.0, device="cuda", dtype=torch.float16) for _ in range(3)]
+    work = torch.empty(1 << 20, device="cuda", dtype=torch.uint8)
+    c = empty_call(empty, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr())
+    need = cs.lib.cutespmm_block_attention_grad_workspace(C.byref(c))
+    assert need <= work.numel()
+    st = cs.lib.cutespmm_block_attention_grad(C.byref(c), q.data_ptr(), c.q_strides, out.data_ptr(), lse.data_ptr(), *(g.data_ptr() for g in grads), work.data_ptr() if need else None, need, None)
+    assert st == 0
+    torch.cuda.synchronize()
+    sizes = [c.batch * c.queries * c.heads * c.dim] + [c.batch * c.keys * c.kv_heads * c.dim] * 2
+    for g, n in zip(grads, sizes):
+        assert not g[:n].any() and (g[n:] == 3.0).all()
