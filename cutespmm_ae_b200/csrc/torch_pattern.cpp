@@ -344,6 +344,9 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
 std::tuple<Tensor, Tensor> autograd_block_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &blocks, int64_t block, const OptTensor &visible, double scale, const OptTensor &pages)
 {
     const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    // a tensor with a tangent need not require a gradient: below here it would lose the tangent without a word
+    for (const Tensor *t : {&q, &k, &v})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "block_attention has no forward-mode derivative");
     if (!graph) {
         at::AutoDispatchBelowADInplaceOrView guard;
         return call_block_attention(q, k, v, blocks, block, visible, scale, pages);

@@ -755,6 +755,28 @@ def test_fake_kernels_give_shapes():
         assert [g.shape for g in torch.ops.cutespmm.block_attention_grad(out, q, k, k, out, lse, blocks, 16, None, 1.0)] == [q.shape, k.shape, k.shape]
 
 
+@pytest.mark.gpu
+def test_no_forward_mode_derivatives():
+    """Refused for all of them, whatever a tangent hangs on: nothing goes on with a tangent of zeros."""
+    torch.manual_seed(19)
+    q, k, v = attention_inputs(torch.bfloat16, 1, 40, 40, 2, 2, 64)
+    blocks = random_blocks(1, 2, 40, 3, 40, 16)
+    ids, table = torch.randint(0, 50, (30,), device="cuda"), torch.randn(50, 16, device="cuda")
+    calls = [(lambda x: ops.block_attention(x, k, v, blocks, 16), q), (lambda x: ops.block_attention(q, x, v, blocks, 16), k), (lambda x: ops.block_attention(q, k, x, blocks, 16), v),
+             (lambda x: ops.embedding(ids, x), table), (lambda x: ops.block_means(x, 16), k), (lambda x: ops.block_scores(x, k), q)]
+    for fn, x in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(fn, (x,), (torch.ones_like(x),))
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+            fn(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+    pages = torch.arange(3, device="cuda", dtype=torch.int32)[None]
+    cache = torch.randn(3, 16, 2, 64, device="cuda").bfloat16()
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        ops.block_attention(torch.autograd.forward_ad.make_dual(q, q), cache, cache, blocks, 16, torch.full((1, 40), 40, device="cuda", dtype=torch.int32), None, pages)
+    with torch.autograd.forward_ad.dual_level():  # without a tangent there is nothing to lose
+        assert torch.equal(ops.block_attention(q, k, v, blocks, 16), ops.block_attention(q, k, v, blocks, 16))
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
