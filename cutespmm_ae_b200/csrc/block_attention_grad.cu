@@ -42,8 +42,10 @@ template <int DP> struct DqSmem {
     static constexpr int kLists = kBars + 192;
 };
 
-// dq of one row by itself: a warp, four dims a lane.
-template <class T> __device__ void exact_dq_row(const AttentionArgs &a, const TileUnion &u, uint32_t b, uint32_t kv, uint32_t t, uint32_t q_of_tile, uint32_t head, float delta)
+// dq of one row by itself: a warp, four dims a lane.  Dims first to end - 1 are written: the others are another warp's, and what it has stored
+// there, or forms again by itself, stays.
+template <class T>
+__device__ void exact_dq_row(const AttentionArgs &a, const TileUnion &u, uint32_t b, uint32_t kv, uint32_t t, uint32_t q_of_tile, uint32_t head, float delta, uint32_t first, uint32_t end)
 {
     const uint32_t lane = threadIdx.x & 31, d = lane * 4;
     const bool on = d < a.dim;
@@ -75,7 +77,7 @@ template <class T> __device__ void exact_dq_row(const AttentionArgs &a, const Ti
             if (on)
                 for (int j = 0; j < 4; ++j) sum[j] = fmaf(ds, to_f32(kr[j]), sum[j]);
         }
-    if (on)
+    if (on && d >= first && d < end)
         for (int j = 0; j < 4; ++j) static_cast<T *>(a.dq)[(((uint64_t)b * a.queries + t) * a.heads + head) * a.dim + d + j] = from_f32<T>(a.scale * sum[j]);
 }
 
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) block_attention_dq_kernel(const
             const uint32_t from = __ffs(left) - 1, rq = __shfl_sync(~0u, q, from), rh = __shfl_sync(~0u, head, from);
             const float rd = __shfl_sync(~0u, delta, from);
             __syncwarp();
-            exact_dq_row<T>(a, u, b, kv, t0 + rq, rq, rh, rd);
+            exact_dq_row<T>(a, u, b, kv, t0 + rq, rq, rh, rd, half * (DP / 2), (half + 1) * (DP / 2));
         }
     }
     tc::fence_before();

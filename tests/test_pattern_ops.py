@@ -777,6 +777,31 @@ def test_no_forward_mode_derivatives():
         assert torch.equal(ops.block_attention(q, k, v, blocks, 16), ops.block_attention(q, k, v, blocks, 16))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_dims_of_a_key_that_is_no_number_do_not_touch_the_others(dim):
+    """An unseen key that is no number in the upper half of its dims: only those dims of dq are formed again."""
+    torch.manual_seed(dim)
+    q, k, v = attention_inputs(torch.bfloat16, 1, 64, 64, 2, 8, dim)
+    blocks = torch.randint(0, 4, (1, 2, 64, 2), device="cuda", dtype=torch.int32)
+    dout = torch.randn(q.shape, device="cuda").bfloat16()
+    pattern = pattern_of(blocks, 16, 64, default_visible(1, 64, 64))
+    rows = ~pattern[..., 40].any(1)[0]  # queries that do not look at key 40
+    want = attention_reference(q, k, v, pattern, 1 / math.sqrt(dim), dout)[1]
+
+    def dq(k):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(ops.block_attention(*leaves, blocks, 16), leaves[0], dout)[0]
+
+    clean = dq(k)
+    k[0, 40, :, dim // 2 + 5] = math.nan
+    runs = [dq(k) for _ in range(8)]
+    for g in runs:
+        assert torch.equal(g[:, rows, :, : dim // 2], clean[:, rows, :, : dim // 2])
+        assert torch.equal(g[:, rows], runs[0][:, rows])
+        within(g[:, rows], want[0][:, rows], want[1][:, rows])
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
