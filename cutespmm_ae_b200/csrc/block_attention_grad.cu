@@ -322,7 +322,7 @@ struct GradLayout {
         delta = take((uint64_t)a.batch * a.heads * a.queries * 4);
         bits_bytes = (uint64_t)a.batch * a.kv_heads * a.num_blocks * words * 4;
         bits = take(bits_bytes);
-        counts = take(tile_rows * 12);  // queries, then the first item, then the first slot of each tile
+        counts = take(tile_rows * 16);  // of each tile: queries, then the first item, then the first slot, then whether sums are formed again
         items = take(max_items * 8);
         totals = take(8);
         partial = take(max_slots * 2 * kKeyTile * (a.dim <= 64 ? 64 : 128) * 4);
@@ -334,7 +334,7 @@ struct TurnArgs {
     AttentionArgs a;
     uint32_t words, tiles, item_queries;
     uint64_t tile_rows;
-    uint32_t *bits, *counts, *first_item, *first_slot;
+    uint32_t *bits, *counts, *first_item, *first_slot, *redo;
     uint2 *items;      // (tile row, which of its items)
     uint32_t *totals;  // items
     float *partial;
@@ -380,7 +380,10 @@ __global__ void __launch_bounds__(256) pattern_count_kernel(TurnArgs p)
     uint32_t n = 0;
     for (uint32_t w = threadIdx.x & 31; w < p.words; w += 32) n += __popc(tile_word(p, row, w));
     n = __reduce_add_sync(~0u, n);
-    if ((threadIdx.x & 31) == 0) p.counts[row] = n;
+    if ((threadIdx.x & 31) == 0) {
+        p.counts[row] = n;
+        p.redo[row] = 0;
+    }
 }
 
 // Work item it: its first query, as a rank among those that name the tile, and how many it takes -- equal parts, whole tiles of rows.
@@ -746,12 +749,15 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const bool is_dk = half != 0;
             const uint32_t d = r, n_items = (p.counts[it.x] + p.item_queries - 1) / p.item_queries;
             const float f = is_dk ? a.scale : 1.f;
+            bool finite = true;
 #pragma unroll 1
             for (uint32_t c = 0; c < 64; c += 32) {
                 uint32_t v[32];
                 tc::ld32(lanes + (is_dk ? kTmemDk : kTmemDv) + c, v);
                 tc::wait_ld();
                 if (d >= a.dim) continue;
+#pragma unroll
+                for (int x = 0; x < 32; ++x) finite = finite && fabsf(__uint_as_float(v[x])) < INFINITY;
                 if (n_items == 1) {
                     T *dst = static_cast<T *>(is_dk ? a.dk : a.dv) + (((uint64_t)b * a.keys + tile * kKeyTile + c) * a.kv_heads + kv) * a.dim + d;
                     const uint32_t n = a.keys > tile * kKeyTile + c ? min(32u, a.keys - tile * kKeyTile - c) : 0u;
@@ -764,6 +770,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                     for (int x = 0; x < 32; ++x) __stcs(dst + x * DP, f * __uint_as_float(v[x]));
                 }
             }
+            if (__any_sync(~0u, !finite) && lane == 0) p.redo[it.x] = 1;
             tc::fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(read);
@@ -779,17 +786,111 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     }
 }
 
+// dk and dv of one key by themselves: a warp, four dims a lane, over the queries that look at the key, in ascending order.
+template <class T> __device__ __forceinline__ void exact_key(const TurnArgs &p, uint32_t b, uint32_t kv, uint32_t key, float (&dk)[4], float (&dv)[4])
+{
+    const AttentionArgs &a = p.a;
+    const uint32_t lane = threadIdx.x & 31, d = lane * 4, group = a.heads / a.kv_heads;
+    const bool on = d < a.dim;
+    const T *kr = key_row<T>(a, a.k, a.k_batch, a.k_key, a.k_head, b, kv, key) + d, *vr = key_row<T>(a, a.v, a.v_batch, a.v_key, a.v_head, b, kv, key) + d;
+    float k[4] = {}, v[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        dk[j] = dv[j] = 0.f;
+        if (on) {
+            k[j] = to_f32(kr[j]);
+            v[j] = to_f32(vr[j]);
+        }
+    }
+    const uint32_t *bits = p.bits + (((uint64_t)b * a.kv_heads + kv) * a.num_blocks + key / a.block) * p.words;
+    for (uint32_t w = 0; w < p.words; w += 32) {
+        const uint32_t mine = w + lane < p.words ? bits[w + lane] : 0u;
+        for (uint32_t some = __ballot_sync(~0u, mine != 0); some; some &= some - 1) {
+            const uint32_t l = __ffs(some) - 1;
+            for (uint32_t word = __shfl_sync(~0u, mine, l); word; word &= word - 1) {
+                const uint32_t t = (w + l) * 32 + __ffs(word) - 1;
+                if (key >= visible_keys(a, b, t)) continue;
+                for (uint32_t head = kv * group; head < (kv + 1) * group; ++head) {
+                    const T *qr = static_cast<const T *>(a.q) + (int64_t)b * a.q_batch + (int64_t)t * a.q_query + (int64_t)head * a.q_head + d;
+                    const T *gr = static_cast<const T *>(a.dout) + (int64_t)b * a.do_batch + (int64_t)t * a.do_query + (int64_t)head * a.do_head + d;
+                    float q[4] = {}, g[4] = {}, s = 0.f, dp = 0.f;
+                    if (on)
+                        for (int j = 0; j < 4; ++j) {
+                            q[j] = to_f32(qr[j]);
+                            g[j] = to_f32(gr[j]);
+                            s = fmaf(q[j], k[j], s);
+                            dp = fmaf(g[j], v[j], dp);
+                        }
+#pragma unroll
+                    for (int x = 16; x; x >>= 1) {
+                        s += __shfl_xor_sync(~0u, s, x);
+                        dp += __shfl_xor_sync(~0u, dp, x);
+                    }
+                    const uint64_t stat = ((uint64_t)b * a.heads + head) * a.queries + t;
+                    const float e = exp2f((s * a.scale - a.lse[stat]) * kLog2e), ds = a.scale * e * (dp - a.delta[stat]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        dk[j] = fmaf(ds, q[j], dk[j]);
+                        dv[j] = fmaf(e, g[j], dv[j]);
+                    }
+                }
+                bool lost = true;  // what is no number stays none
+                for (int j = 0; j < 4; ++j) lost = lost && dk[j] != dk[j] && dv[j] != dv[j];
+                if (__all_sync(~0u, lost || !on)) return;
+            }
+        }
+    }
+}
+
 // Key tiles that no query names are zero; the partial sums of those with several work items are added in order.  Eight blocks of threads a tile.
+// In a tile that has a sum which is not finite, a warp takes a key: the products multiply every gathered row of q and dout with all 64 keys, and 0 times
+// a row that is no number is not 0, so such a key is formed again from the queries that look at it.
 template <class T, int DP> __global__ void __launch_bounds__(256) dkv_join_kernel(TurnArgs p)
 {
     ptx::grid_wait();
     ptx::grid_release();
     const AttentionArgs &a = p.a;
     const uint32_t row = blockIdx.x, items = (p.counts[row] + p.item_queries - 1) / p.item_queries;
-    if (items == 1) return;
+    const bool redo = p.redo[row] != 0;
+    if (items == 1 && !redo) return;
     const uint32_t tile = row % p.tiles, bh = row / p.tiles, b = bh / a.kv_heads, kv = bh % a.kv_heads;
     const uint32_t n = min(kKeyTile, a.keys - tile * kKeyTile);
     const float *src = p.partial + (uint64_t)p.first_slot[row] * 2 * kKeyTile * DP;
+    if (redo) {
+        const uint32_t d = (threadIdx.x & 31) * 4;
+        for (uint32_t key = blockIdx.y * 8 + (threadIdx.x >> 5); key < n; key += 8 * gridDim.y) {
+            const uint64_t at = (((uint64_t)b * a.keys + tile * kKeyTile + key) * a.kv_heads + kv) * a.dim + d;
+            T *to_dk = static_cast<T *>(a.dk) + at, *to_dv = static_cast<T *>(a.dv) + at;
+            float dk[4] = {}, dv[4] = {};
+            if (d < a.dim && items == 1) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dk[j] = to_f32(to_dk[j]);
+                    dv[j] = to_f32(to_dv[j]);
+                }
+            } else if (d < a.dim)
+                for (uint32_t k = 0; k < items; ++k) {
+                    const float *part = src + (uint64_t)k * 2 * kKeyTile * DP + key * DP + d;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        dv[j] += part[j];
+                        dk[j] += part[kKeyTile * DP + j];
+                    }
+                }
+            bool finite = true;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) finite = finite && fabsf(dk[j]) < INFINITY && fabsf(dv[j]) < INFINITY;
+            if (!__all_sync(~0u, finite)) exact_key<T>(p, b, kv, tile * kKeyTile + key, dk, dv);
+            if (d < a.dim) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    to_dk[j] = from_f32<T>(dk[j]);
+                    to_dv[j] = from_f32<T>(dv[j]);
+                }
+            }
+        }
+        return;
+    }
     for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < 2 * n * (DP / 4); i += 256 * gridDim.y) {
         const uint32_t d = i % (DP / 4) * 4, key = i / (DP / 4) % n, is_dk = i / (DP / 4) / n;
         if (d >= a.dim) continue;
@@ -843,6 +944,7 @@ template <class T, int DP> cudaError_t launch_grad(AttentionArgs a, int sm_count
     p.counts = reinterpret_cast<uint32_t *>(w + l.counts);
     p.first_item = p.counts + l.tile_rows;
     p.first_slot = p.first_item + l.tile_rows;
+    p.redo = p.first_slot + l.tile_rows;
     p.items = reinterpret_cast<uint2 *>(w + l.items);
     p.totals = reinterpret_cast<uint32_t *>(w + l.totals);
     p.partial = reinterpret_cast<float *>(w + l.partial);

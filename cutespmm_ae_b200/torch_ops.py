@@ -251,7 +251,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     q: [batch, queries, heads, dim]; k, v: [batch, keys, kv_heads, dim]; float16 or bfloat16, dim a multiple of 8 up to 128, heads a
     multiple of kv_heads (up to 128 times).  blocks: int32 [batch, kv_heads, queries, count], count at most 128, a set of blocks of `block` keys (16, 32, 64,
     128) for each query, as `select_blocks` returns it: any order, an index outside the keys names nothing, a repeated one counts once.
-    visible: as in `select_blocks`.  Keys that a query does not see have no effect on it, whatever their values.
+    visible: as in `select_blocks`.  Keys that a query does not look at have no effect on it, nor it on their gradients, whatever the values of either.
 
     A paged cache: pages int32 [batch, pages of a sequence], k and v [number of pages, block, kv_heads, dim]; block j of sequence b is
     page pages[b, j] (an entry that is no page holds no keys), and visible says how many keys are written.  No gradient then.

@@ -326,8 +326,9 @@ int cutespmm_select_blocks(const float *scores_dev, const int64_t s_strides[3], 
  * heads x dim, contiguous; lse[b][h][t]: the logarithm of the sum of exponentials (-infinity where there are none). */
 int cutespmm_block_attention(const cutespmm_block_attention_t *args, void *out_dev, float *lse_dev, void *stream);
 /* Gradients with respect to q, k and v (contiguous, shaped like them) from out, lse and dout (dout_strides as q's).  Not for a paged
- * cache.  Sums have a fixed order.  P and P (dout v - <dout, out>) are rounded to the 16-bit type on the way, so the latter must stay
- * within fp16's range where that is the type.  workspace: cutespmm_block_attention_grad_workspace() bytes, 256-byte aligned, not shared with a
+ * cache.  Sums have a fixed order.  P and P (dout v - <dout, out>) are rounded to the 16-bit type on the way; where the latter leave
+ * fp16's range, or a key or a query's row is no number, the sums concerned are formed again in fp32 from the pairs that look at each
+ * other (slowly: a warp a row or key).  So nothing reaches the gradient of a key from a query that does not look at it.  workspace: cutespmm_block_attention_grad_workspace() bytes, 256-byte aligned, not shared with a
  * call that may overlap. */
 uint64_t cutespmm_block_attention_grad_workspace(const cutespmm_block_attention_t *args);
 int cutespmm_block_attention_grad(const cutespmm_block_attention_t *args, const void *dout_dev, const int64_t dout_strides[3],

@@ -802,6 +802,57 @@ def test_dims_of_a_key_that_is_no_number_do_not_touch_the_others(dim):
         within(g[:, rows], want[0][:, rows], want[1][:, rows])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("form", [(1, 70, 128, 2, 4, 64, 16, 3), (1, 300, 300, 1, 8, 128, 64, 2), (2, 90, 130, 2, 3, 72, 32, 2), (1, 130, 256, 1, 1, 128, 128, 1), (1, 1500, 1500, 1, 8, 64, 64, 4)])
+@pytest.mark.parametrize("what", ["q", "dout", "both"])
+def test_rows_that_are_no_numbers_reach_no_key_they_do_not_look_at(dtype, form, what):
+    """NaN and infinities in q or dout of two queries: dk and dv of the keys they do not look at are those without them, also inside a tile of
+    64 keys -- another block of it, or the keys behind the last that they see -- and where a tile's sums come in parts."""
+    batch, queries, keys, kv, group, dim, block, count = form
+    torch.manual_seed(queries + dim)
+    q, k, v = attention_inputs(dtype, batch, queries, keys, kv, group, dim)
+    blocks = random_blocks(batch, kv, queries, count, keys, block)
+    blocks[..., 0] = 0  # many work items for the first tile of the longest form
+    bad = [40, 700] if queries > 1000 else [queries // 2, queries // 2 + 1]
+    for t in bad:
+        blocks[:, :, t] = -1
+        blocks[:, :, t, 0] = (keys - queries + t) // block  # the block that holds the last key it sees
+    pattern = pattern_of(blocks, block, keys, default_visible(batch, queries, keys))
+    dout = torch.randn(q.shape, device="cuda").to(dtype)
+    want = attention_reference(q, k, v, pattern, 1 / math.sqrt(dim), dout)
+    if what != "dout":
+        q[:, bad[0], :, dim // 3] = math.nan
+        q[:, bad[1], 0, 0] = math.inf
+    if what != "q":
+        dout[:, bad[0], -1] = math.nan
+        dout[:, bad[1], :, 1] = -math.inf
+    free = ~pattern[:, :, bad].any(2).transpose(1, 2)  # [batch, keys, kv]
+    tiles = [(keys - queries + t) // 64 * 64 for t in bad]
+    assert any(free[:, i : i + 64].any() and not free[:, i : i + 64].all() for i in tiles)  # a tile of 64 keys of which they see a part
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.block_attention(*leaves, blocks, block), leaves, dout)
+    others = torch.ones(queries, device="cuda", dtype=torch.bool)
+    others[bad] = False
+    within(grads[0][:, others], want[1][0][:, others], want[1][1][:, others])
+    for g, (w, bound) in zip(grads[1:], want[2:]):
+        within(g[free], w[free], bound[free])
+    assert not torch.isfinite(grads[1][~free]).all() and not torch.isfinite(grads[2][~free]).all()  # while what they look at shows it
+    again = torch.autograd.grad(ops.block_attention(*leaves, blocks, block), leaves, dout)
+    for a, b in zip(grads, again):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+@pytest.mark.gpu
+def test_gradients_whose_inner_products_leave_the_range_of_half():
+    """dout v beyond 65504, as a scaled loss makes it: dS has no fp16 form there, but dq, dk and dv do."""
+    torch.manual_seed(23)
+    q, k, v = attention_inputs(torch.float16, 1, 200, 200, 2, 4, 64)
+    blocks = random_blocks(1, 2, 200, 3, 200, 16)
+    got = check_attention(q, k, v * 100, blocks, 16, scale=1e-3, dout=(torch.randn(q.shape, device="cuda") * 300).half())
+    assert all(torch.isfinite(g).all() for g in got)
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
