@@ -55,10 +55,13 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, 
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// Reads a status word that is a __device__ variable of the calling file on the current device and clears it where it is set.
+// Reads a status word that is a __device__ variable of the calling file on the current device and clears it where it is set, once all that
+// is queued on the device is done: the copy alone would not wait for streams that do not wait for the default one.  What another thread's
+// kernels write between copy and clear is part of what this read reports: it reports nothing only where it clears nothing.
 template <class Symbol> cudaError_t read_status(Symbol &symbol, uint32_t *word)
 {
-    cudaError_t e = cudaMemcpyFromSymbol(word, symbol, sizeof *word);
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(word, symbol, sizeof *word);
     const uint32_t zero = 0;
     if (e == cudaSuccess && *word) e = cudaMemcpyToSymbol(symbol, &zero, sizeof zero);
     return e;

@@ -62,10 +62,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
     return ok != 0;
 }
 // Bounded wait for the phase with the given parity.  false = gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32_t limit = kSpinLimit)
 {
     if (mbar_try_wait(bar, parity)) return true;  // the common case: the phase is already complete
-    for (uint32_t i = 1; i < kSpinLimit; ++i)
+    for (uint32_t i = 1; i < limit; ++i)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }

@@ -853,6 +853,30 @@ def test_gradients_whose_inner_products_leave_the_range_of_half():
     assert all(torch.isfinite(g).all() for g in got)
 
 
+@pytest.mark.gpu
+def test_the_status_read_waits_for_every_stream():
+    side = torch.cuda.Stream()
+    done = torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        done.record()
+    assert ops.pattern_status() == 0
+    assert done.query()
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported_once(tmp_path):
+    """The kernels' wait with a limit of a few polls on a barrier that nothing arrives at: it ends, the word is read behind it, and cleared."""
+    import subprocess
+    from conftest import ROOT
+
+    exe = tmp_path / "status_driver"
+    subprocess.run([cs._build.NVCC, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", f"-I{cs._build.CSRC}", str(ROOT / "tests" / "cpp" / "status_driver.cu"), "-o", str(exe)],
+                   check=True, capture_output=True, text=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0 and res.stdout.strip() == "ran out 1, read again 0, arrived 0", res.stdout + res.stderr
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
