@@ -594,7 +594,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
             v.y = tc::round2<T>(o.z * inv, o.w * inv);
             *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (((uint64_t)b * a.queries + t) * a.heads + head) * a.dim + d) = v;
         }
-        if (d == 0) a.lse[((uint64_t)b * a.heads + head) * a.queries + t] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        // a sum that is no number (a seen key that is none) makes lse none, as it makes out
+        if (d == 0) a.lse[((uint64_t)b * a.heads + head) * a.queries + t] = sum != 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
     if (ranks > 1) cluster_sync();  // a peer may still be reading this block's shared memory
 }

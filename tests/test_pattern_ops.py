@@ -877,6 +877,25 @@ def test_a_wait_that_runs_out_is_reported_once(tmp_path):
     assert res.returncode == 0 and res.stdout.strip() == "ran out 1, read again 0, arrived 0", res.stdout + res.stderr
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 4, 5])
+def test_a_seen_key_that_is_no_number_shows(queries):
+    """Few queries and many give the same for a row whose scores are no numbers: out, lse and dq of that row are none either."""
+    torch.manual_seed(20)
+    q, k, v = attention_inputs(torch.bfloat16, 1, queries, 64, 1, 4, 64)
+    blocks = torch.zeros(1, 1, queries, 2, device="cuda", dtype=torch.int32)
+    blocks[..., 1] = 2
+    visible = torch.full((1, queries), 64, device="cuda", dtype=torch.int32)
+    k[0, 3, 0, 7] = math.nan
+    out, lse = torch.ops.cutespmm.block_attention(q, k, v, blocks, 16, visible, 0.125, None)
+    assert out.isnan().all() and lse.isnan().all()
+    dq, dk, dv = torch.ops.cutespmm.block_attention_grad(torch.ones_like(q), q, k, v, out, lse, blocks, 16, visible, 0.125)
+    named = torch.zeros(64, device="cuda", dtype=torch.bool)
+    named[0:16] = named[32:48] = True
+    assert dq.isnan().all() and dk[0, named].isnan().all() and dv[0, named].isnan().all()
+    assert not dk[0, ~named].any() and not dv[0, ~named].any()
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
