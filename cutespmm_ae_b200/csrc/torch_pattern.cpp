@@ -26,7 +26,11 @@ int dtype_of(const Tensor &t)
         default: return -1;
     }
 }
-uint32_t u32(int64_t v) { return (uint32_t)v; }
+uint32_t u32(int64_t v)
+{
+    TORCH_CHECK_VALUE(v >= 0 && v <= (int64_t)UINT32_MAX, "a size of ", v, " is beyond 32 bits");
+    return (uint32_t)v;
+}
 Tensor empty_like_of(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false).memory_format(at::MemoryFormat::Contiguous)); }
 Tensor empty_like_of(at::IntArrayRef sizes, const Tensor &like) { return empty_like_of(sizes, like, like.scalar_type()); }
 Tensor scratch(uint64_t bytes, const Tensor &like) { return bytes ? empty_like_of({(int64_t)bytes}, like, at::kByte) : Tensor(); }
@@ -152,7 +156,7 @@ Tensor op_select_blocks(const Tensor &scores, int64_t count, int64_t block, int6
     TORCH_CHECK_VALUE(scores.dim() == 4 && scores.scalar_type() == at::kFloat, "scores must be a [batch, kv_heads, queries, blocks] float32 tensor");
     check_block(block);
     TORCH_CHECK_VALUE(keys >= 0 && keys < (int64_t)1 << 28 && scores.size(3) == (keys + block - 1) / block, "scores must have a column per block of the ", keys, " keys");
-    TORCH_CHECK_VALUE(count >= 0 && first >= 0 && last >= 0 && first + last <= count, "first + last must not exceed count");
+    TORCH_CHECK_VALUE(count >= 0 && first >= 0 && last >= 0 && first <= count && last <= count - first, "first + last must not exceed count");
     check_visible(visible, scores.size(0), scores.size(2));
     want_cuda(scores, {visible});
     const c10::cuda::CUDAGuard guard(scores.device());

@@ -896,6 +896,15 @@ def test_a_seen_key_that_is_no_number_shows(queries):
     assert not dk[0, ~named].any() and not dv[0, ~named].any()
 
 
+@pytest.mark.gpu
+def test_numbers_beyond_32_bits_are_refused():
+    """Not cut down to what is left of them: a result without rows shows it without memory."""
+    none = torch.zeros(0, 1, 1, 4, device="cuda")
+    refused("beyond 32 bits", ops.select_blocks, none, 2**32 + 5, 16, 64)
+    refused("first \\+ last", ops.select_blocks, none, 3, 16, 64, None, 2**62, 2**62)
+    refused("beyond 32 bits|2\\^31", torch.ops.cutespmm.embedding_grad, torch.zeros(3, device="cuda", dtype=torch.int32), torch.zeros(3, 0, device="cuda"), 2**40, 1.0)
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
