@@ -92,7 +92,7 @@ struct Operand {
             t = x.contiguous();
             if (!fits()) t = x.clone(at::MemoryFormat::Contiguous);  // contiguous, but off the 16-byte grid
         }
-        for (int i = 0; i < 3; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        for (int i = 0; i < 3; ++i) strides[i] = t.numel() && t.size(i) > 1 ? t.stride(i) : 0;  // without elements any strides will do
     }
     bool fits() const
     {

@@ -905,6 +905,21 @@ def test_numbers_beyond_32_bits_are_refused():
     refused("beyond 32 bits|2\\^31", torch.ops.cutespmm.embedding_grad, torch.zeros(3, device="cuda", dtype=torch.int32), torch.zeros(3, 0, device="cuda"), 2**40, 1.0)
 
 
+@pytest.mark.gpu
+def test_empty_operands_off_the_grid():
+    """Slices without elements, of tensors whose strides are no multiples of 8."""
+    q, wide = (torch.randn(2, n, h, 75, device="cuda").half() for n, h in ((9, 2), (33, 1)))
+    k = wide[:, :0, :, 3:67]
+    blocks = torch.zeros(2, 1, 9, 2, device="cuda", dtype=torch.int32)
+    assert k.stride(0) % 8 and not ops.block_attention(q[..., 3:67], k, k, blocks, 16).any()
+    leaves = [t.detach().requires_grad_(True) for t in (q[..., 3:67], k, k)]
+    grads = torch.autograd.grad(ops.block_attention(*leaves, blocks, 16).sum(), leaves)
+    assert not grads[0].any() and grads[1].shape == grads[2].shape == (2, 0, 1, 64)
+    assert ops.block_means(k, 16).shape == (2, 0, 1, 64)
+    assert ops.block_scores(q[:, :0, :, 3:67], wide[..., 3:67]).shape == (2, 1, 0, 33)
+    assert ops.block_scores(q[..., 3:67], k).shape == (2, 1, 9, 0)
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
