@@ -406,6 +406,7 @@ cudaError_t launch_block_means(const MeansArgs &a, cudaStream_t s)
 cudaError_t launch_block_scores(const ScoresArgs &a, int sm_count, cudaStream_t s)
 {
     if (!a.batch || !a.queries || !a.kv_heads || !a.blocks) return cudaSuccess;
+    if (!a.heads) return cudaMemsetAsync(a.scores, 0, (uint64_t)a.batch * a.kv_heads * a.queries * a.blocks * 4, s);  // sums of nothing
     const bool bf16 = a.dtype == CUTESPMM_BF16;
     CUtensorMap q_map, m_map;
     cudaError_t e = tc::make_map(&q_map, bf16, a.q, a.dim, a.heads, a.queries, a.batch, a.q_head, a.q_query, a.q_batch, kScoreRows);

@@ -156,7 +156,7 @@ int cutespmm_block_scores(int dtype, const void *q_dev, const int64_t q_strides[
         return refuse(CUTESPMM_EINVAL, "q and means must be 16-byte aligned, their strides multiples of 8 elements");
     if (blocks > 65536) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65536 blocks of keys");
     if (((uint64_t)(blocks + 255) / 256 * ((queries + 127) / 128) * batch * kv_heads) >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "too many queries and blocks for one call");
-    if (batch && queries && heads && blocks && (!q_dev || !means_dev || !scores_dev)) return refuse(CUTESPMM_EINVAL, "q, means or scores is NULL");
+    if (batch && queries && blocks && ((heads && (!q_dev || !means_dev)) || !scores_dev)) return refuse(CUTESPMM_EINVAL, "q, means or scores is NULL");
     if (!on_grid(scores_dev, 4)) return refuse(CUTESPMM_EINVAL, kOffElements);
     int dev = -1, sms = 0;
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;

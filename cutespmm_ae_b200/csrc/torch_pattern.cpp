@@ -144,7 +144,6 @@ Tensor op_block_scores(const Tensor &q, const Tensor &means)
     const Operand x(q), m(means);
     Tensor scores = empty_like_of({q.size(0), means.size(2), q.size(1), means.size(1)}, q, at::kFloat);
     if (scores.numel() == 0) return scores;
-    if (q.size(2) == 0) return scores.zero_();
     check_status(cutespmm_block_scores(dtype_of(q), ptr<void>(x.t), x.strides, ptr<void>(m.t), m.strides, u32(q.size(0)), u32(q.size(1)), u32(q.size(2)), u32(means.size(2)),
                                        u32(means.size(1)), u32(q.size(3)), ptr<float>(scores), stream_of(q)));
     return scores;

@@ -1023,3 +1023,15 @@ def test_empty_gradients_of_the_c_abi(empty):
     sizes = [c.batch * c.queries * c.heads * c.dim] + [c.batch * c.keys * c.kv_heads * c.dim] * 2
     for g, n in zip(grads, sizes):
         assert not g[:n].any() and (g[n:] == 3.0).all()
+
+
+@pytest.mark.gpu
+def test_scores_of_no_heads_are_zero():
+    import ctypes as C
+
+    s3 = (C.c_int64 * 3)(64, 64, 64)
+    means, scores = torch.randn(384, device="cuda").half(), torch.full((2 * 5 * 3 + 2,), 7.0, device="cuda")
+    assert cs.lib.cutespmm_block_scores(1, None, s3, means.data_ptr(), s3, 2, 5, 0, 1, 3, 64, scores.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert not scores[:30].any() and (scores[30:] == 7.0).all()
+    assert not ops.block_scores(torch.zeros(2, 5, 0, 64, device="cuda").half(), means.view(2, 3, 1, 64)).any()
