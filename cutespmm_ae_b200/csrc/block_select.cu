@@ -28,7 +28,7 @@ template <class T> __global__ void __launch_bounds__(kMeanWarps * 32) block_mean
     ptx::grid_wait();
     ptx::grid_release();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, packs = a.dim / 8;
-    const uint32_t col = blockIdx.x * 32 + lane, blk = blockIdx.y, b = blockIdx.z;
+    const uint32_t col = blockIdx.y * 32 + lane, blk = blockIdx.x, b = blockIdx.z;
     const uint32_t head = col / packs, d = col % packs * 8;
     const bool on = head < a.kv_heads;
     const uint32_t keys = a.lengths ? (uint32_t)min(max(a.lengths[b], 0), (int)a.keys) : a.keys;
@@ -46,7 +46,7 @@ template <class T> __global__ void __launch_bounds__(kMeanWarps * 32) block_mean
     for (int j = 0; j < 8; ++j) part[warp][lane][j] = acc[j];
     __syncthreads();
     // thread t adds column t of the 256 over the warps
-    const uint32_t l = threadIdx.x >> 3, j = threadIdx.x & 7, out_col = blockIdx.x * 32 + l;
+    const uint32_t l = threadIdx.x >> 3, j = threadIdx.x & 7, out_col = blockIdx.y * 32 + l;
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kMeanWarps; ++w) sum += part[w][l][j];
@@ -398,7 +398,7 @@ template <int R, int WARPS> __global__ void __launch_bounds__(WARPS == 1 ? 128 :
 cudaError_t launch_block_means(const MeansArgs &a, cudaStream_t s)
 {
     if (!a.batch || !a.blocks || !a.kv_heads || !a.dim) return cudaSuccess;
-    const dim3 grid((a.kv_heads * (a.dim / 8) + 31) / 32, a.blocks, a.batch);
+    const dim3 grid(a.blocks, (a.kv_heads * (a.dim / 8) + 31) / 32, a.batch);
     return a.dtype == CUTESPMM_BF16 ? launch_overlapped(block_means_kernel<__nv_bfloat16>, grid, dim3(kMeanWarps * 32), 0, s, a)
                                     : launch_overlapped(block_means_kernel<__half>, grid, dim3(kMeanWarps * 32), 0, s, a);
 }

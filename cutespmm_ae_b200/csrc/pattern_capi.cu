@@ -54,6 +54,8 @@ int check_blocks(int dtype, uint32_t batch, uint32_t rows, uint32_t heads, uint3
     return CUTESPMM_OK;
 }
 bool block_size_ok(uint32_t block) { return block == 16 || block == 32 || block == 64 || block == 128; }
+constexpr uint32_t kMostBlocks = 65536;
+const char *const kTooManyBlocks = "at most 65536 blocks of keys";
 const char *const kBlockSizes = "block must be 16, 32, 64 or 128";
 
 // Checks a call's description and turns it into the kernels' arguments.
@@ -69,8 +71,9 @@ int to_args(const cutespmm_block_attention_t *d, AttentionArgs &a)
     if (d->keys >> 28) return refuse(CUTESPMM_EUNSUPPORTED, "more than 2^28 - 1 keys");
     if (d->heads / d->kv_heads > 128) return refuse(CUTESPMM_EUNSUPPORTED, "at most 128 query heads for each head of keys");
     if (!fits_grid((uint64_t)d->batch * 4)) return refuse(CUTESPMM_EUNSUPPORTED, "batch must be at most 16383");
+    if (!fits_grid((uint64_t)d->kv_heads * ((d->heads / d->kv_heads + 7) / 8))) return refuse(CUTESPMM_EUNSUPPORTED, "too many heads: kv_heads for every eight of a group must be at most 65535");
     const uint32_t blocks = (d->keys + d->block - 1) / d->block;
-    if (blocks > 65536) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65536 blocks of keys");
+    if (blocks > kMostBlocks) return refuse(CUTESPMM_EUNSUPPORTED, kTooManyBlocks);
     if (d->pages && (uint64_t)d->page_cols * d->block != d->keys) return refuse(CUTESPMM_EINVAL, "keys must be page_cols * block for a paged cache");
     if (d->pages && d->num_pages >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "more than 2^31 - 1 pages");
     const bool work = d->batch && d->queries && d->heads;
@@ -136,7 +139,7 @@ int cutespmm_block_means(int dtype, const void *k_dev, const int64_t k_strides[3
     if (st != CUTESPMM_OK) return st;
     if (!block_size_ok(block)) return refuse(CUTESPMM_EINVAL, kBlockSizes);
     const uint32_t blocks = (keys + block - 1) / block;
-    if (!fits_grid(blocks)) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65535 blocks of keys");
+    if (blocks > kMostBlocks) return refuse(CUTESPMM_EUNSUPPORTED, kTooManyBlocks);
     if (!k_strides || !aligned(k_dev, k_strides)) return refuse(CUTESPMM_EINVAL, "k must be 16-byte aligned, its strides multiples of 8 elements");
     if (batch && blocks && (!k_dev || !means_dev)) return refuse(CUTESPMM_EINVAL, "k or means is NULL");
     if (!on_grid(lengths_dev, 4) || !on_grid(means_dev, 2)) return refuse(CUTESPMM_EINVAL, kOffElements);
@@ -154,7 +157,7 @@ int cutespmm_block_scores(int dtype, const void *q_dev, const int64_t q_strides[
     if (st != CUTESPMM_OK) return st;
     if (!q_strides || !means_strides || !aligned(q_dev, q_strides) || !aligned(means_dev, means_strides))
         return refuse(CUTESPMM_EINVAL, "q and means must be 16-byte aligned, their strides multiples of 8 elements");
-    if (blocks > 65536) return refuse(CUTESPMM_EUNSUPPORTED, "at most 65536 blocks of keys");
+    if (blocks > kMostBlocks) return refuse(CUTESPMM_EUNSUPPORTED, kTooManyBlocks);
     if (((uint64_t)(blocks + 255) / 256 * ((queries + 127) / 128) * batch * kv_heads) >> 31) return refuse(CUTESPMM_EUNSUPPORTED, "too many queries and blocks for one call");
     if (batch && queries && blocks && ((heads && (!q_dev || !means_dev)) || !scores_dev)) return refuse(CUTESPMM_EINVAL, "q, means or scores is NULL");
     if (!on_grid(scores_dev, 4)) return refuse(CUTESPMM_EINVAL, kOffElements);

@@ -217,7 +217,7 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> 
 def block_means(k: torch.Tensor, block: int, lengths: torch.Tensor | None = None) -> torch.Tensor:
     """Mean key of every block of `block` (16, 32, 64, 128) keys: k [batch, keys, kv_heads, dim] (float16 or bfloat16, dim a multiple of 8 up
     to 128) -> [batch, ceil(keys / block), kv_heads, dim].  The last block's mean is over the keys it has; with `lengths` (int32, [batch]) only
-    the first lengths[b] keys of a sequence count, and a block without any has mean zero.  No gradient."""
+    the first lengths[b] keys of a sequence count, and a block without any has mean zero.  At most 65536 blocks.  No gradient."""
     if torch.compiler.is_compiling():
         return torch.ops.cutespmm.block_means(k, block, lengths)
     return _native.op_block_means(k, block, lengths)
@@ -225,7 +225,7 @@ def block_means(k: torch.Tensor, block: int, lengths: torch.Tensor | None = None
 
 def block_scores(q: torch.Tensor, means: torch.Tensor) -> torch.Tensor:
     """Scores [batch, kv_heads, queries, blocks] (float32) of queries [batch, queries, heads, dim] against mean keys: the dot products of
-    the query heads that share a head of keys, added up.  No gradient: a selection has none."""
+    the query heads that share a head of keys, added up.  At most 65536 blocks.  No gradient: a selection has none."""
     if torch.compiler.is_compiling():
         return torch.ops.cutespmm.block_scores(q, means)
     return _native.op_block_scores(q, means)
@@ -234,7 +234,7 @@ def block_scores(q: torch.Tensor, means: torch.Tensor) -> torch.Tensor:
 def select_blocks(scores: torch.Tensor, count: int, block: int, keys: int, visible: torch.Tensor | None = None, first: int = 1, last: int = 1) -> torch.Tensor:
     """The blocks each query attends to: int32 [batch, kv_heads, queries, count], ascending, -1 behind the last.  Chosen are the `first` first
     and the `last` last of the blocks that the query sees, then those it sees of the highest scores (of equal ones the lowest index; a
-    block whose score is NaN or -infinity only if it is one of the first or last).
+    block whose score is NaN or -infinity only if it is one of the first or last).  At most 16384 blocks to choose from.
 
     visible: int32 [batch, queries], how many keys each query sees (the first that many; 0 for a padded position); None: causal, the last
     query sees all `keys` of them, each before it one less."""
@@ -249,7 +249,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: t
     sees none.  scale is positive and defaults to 1 / sqrt(dim).
 
     q: [batch, queries, heads, dim]; k, v: [batch, keys, kv_heads, dim]; float16 or bfloat16, dim a multiple of 8 up to 128, heads a
-    multiple of kv_heads (up to 128 times).  blocks: int32 [batch, kv_heads, queries, count], count at most 128, a set of blocks of `block` keys (16, 32, 64,
+    multiple of kv_heads (up to 128 times), batch up to 16383, up to 65536 blocks of keys.  blocks: int32 [batch, kv_heads, queries, count], count at most 128, a set of blocks of `block` keys (16, 32, 64,
     128) for each query, as `select_blocks` returns it: any order, an index outside the keys names nothing, a repeated one counts once.
     visible: as in `select_blocks`.  Keys that a query does not look at have no effect on it, nor it on their gradients, whatever the values of either.
 

@@ -288,6 +288,9 @@ int cutespmm_embedding_grad(int dtype, const void *dout_dev, uint64_t ld_dout, c
  * 128.  q, k, v and the means are fp16 or bf16.  Operands are [batch][row][head][dim] with strides in elements, dim contiguous,
  * strides multiples of 8 and pointers 16-byte aligned.  So are out, dq, dk and dv.
  *
+ * Limits (CUTESPMM_EUNSUPPORTED beyond): fewer than 2^28 queries and keys, 65536 blocks of keys (16384 to select from), batch * kv_heads up to
+ * 65535; attention itself 128 query heads to a head of keys, 128 blocks per query, batch up to 16383.
+ *
  * visible[b][t]: how many keys query t of sequence b sees -- the first that many; 0: the query is padding and its output zero;
  * clamped to [0, keys].  NULL: causal, the last query sees every key (query t sees keys - queries + 1 + t). */
 typedef struct {

@@ -1035,3 +1035,34 @@ def test_scores_of_no_heads_are_zero():
     torch.cuda.synchronize()
     assert not scores[:30].any() and (scores[30:] == 7.0).all()
     assert not ops.block_scores(torch.zeros(2, 5, 0, 64, device="cuda").half(), means.view(2, 3, 1, 64)).any()
+
+
+@pytest.mark.gpu
+def test_as_many_blocks_as_scores_and_attention_take():
+    """65536 blocks have means, scores and attention; one more is refused by all three."""
+    torch.manual_seed(24)
+    k = torch.randn(1, 65536 * 16, 1, 8, device="cuda").half()
+    means = ops.block_means(k, 16)
+    parts = k.double().view(65536, 16, 8)
+    within(means[0, :, 0], parts.mean(1), parts.mean(1).abs() * half_step(k.dtype) + parts.abs().mean(1) * 19 * U32 + tiny(k.dtype))
+    q = torch.randn(1, 6, 1, 8, device="cuda").half()
+    assert ops.block_scores(q, means).shape == (1, 1, 6, 65536)
+    blocks = torch.tensor([65535, 0, 40000], device="cuda", dtype=torch.int32).expand(1, 1, 6, 3)
+    see = torch.full((1, 6), k.shape[1], device="cuda", dtype=torch.int32)
+    keys = torch.cat([k[:, j * 16 : j * 16 + 16] for j in (0, 40000, 65535)], 1)
+    few = torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32).expand(1, 1, 6, 3)
+    (want,) = attention_reference(q, keys, keys, pattern_of(few, 16, 48, torch.full((1, 6), 48, device="cuda")), 1 / math.sqrt(8))
+    within(ops.block_attention(q, k, k, blocks, 16, see), *want)
+    more = torch.zeros(1, 65536 * 16 + 1, 1, 8, device="cuda").half()
+    refused("65536", ops.block_means, more, 16)
+    refused("65536", ops.block_scores, q, torch.zeros(1, 65537, 1, 8, device="cuda").half())
+    refused("65536", ops.block_attention, q, more, more, blocks, 16, see)
+
+
+def test_grids_that_are_too_large_are_refused():
+    import ctypes as C
+
+    p = 1 << 20
+    many = attention_call(p, p, p, p, 16, 4, 9000 * 64, kv_heads=9000)
+    assert cs.lib.cutespmm_block_attention(C.byref(many), p, p, None) == -4
+    assert cs.lib.cutespmm_block_attention_grad_workspace(C.byref(many)) == 0
