@@ -11,6 +11,7 @@
 #include "pattern_ops.hpp"
 #include "ptx.cuh"
 #include "tc16.cuh"
+#include "tmap.hpp"
 
 namespace cutespmm {
 namespace {
@@ -447,24 +448,12 @@ namespace tc {
 cudaError_t make_map(CUtensorMap *out, bool bf16, const void *p, uint32_t dim, uint32_t heads, uint32_t rows, uint32_t outer, int64_t head_stride, int64_t row_stride,
                      int64_t outer_stride, uint32_t box_rows, uint32_t box_heads)
 {
-    using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                       CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeTiledFn enc = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
-        return reinterpret_cast<EncodeTiledFn>(f);
-    }();
-    if (!enc) return cudaErrorNotSupported;
     // the stride of an extent of one is never used, but has to be one that a map can hold
     auto bytes = [](int64_t stride, uint32_t extent) { return (cuuint64_t)(extent > 1 ? stride * 2 : 16); };
     const cuuint64_t dims[4] = {dim, heads, rows, outer};
     const cuuint64_t strides[3] = {bytes(head_stride, heads), bytes(row_stride, rows), bytes(outer_stride, outer)};
-    const cuuint32_t box[4] = {64, box_heads, box_rows, 1}, one[4] = {1, 1, 1, 1};
-    return enc(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
+    const cuuint32_t box[4] = {64, box_heads, box_rows, 1};
+    return encode_tiled(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 }  // namespace tc

@@ -920,6 +920,44 @@ def test_empty_operands_off_the_grid():
     assert ops.block_scores(q[..., 3:67], k).shape == (2, 1, 9, 0)
 
 
+def in_a_new_thread(fn):
+    import threading
+
+    got = []
+
+    def body():
+        try:
+            got.append(fn())
+        except Exception as e:  # noqa: BLE001 -- shown by the thread that waits
+            got.append(e)
+
+    t = threading.Thread(target=body)
+    t.start()
+    t.join()
+    if isinstance(got[0], Exception):
+        raise got[0]
+    return got[0]
+
+
+@pytest.mark.gpu
+def test_the_first_call_of_a_thread():
+    """A thread that has asked nothing of the device before, with memory that torch's allocator holds already."""
+    torch.manual_seed(26)
+    q, k, v = attention_inputs(torch.bfloat16, 1, 70, 70, 2, 8, 64)
+    blocks = random_blocks(1, 2, 70, 3, 70, 16)
+    out, lse = torch.ops.cutespmm.block_attention(q, k, v, blocks, 16, None, 0.125, None)
+    dout = torch.randn_like(q)
+    table, ids = torch.randn(50, 16, device="cuda"), torch.randint(0, 50, (30,), device="cuda")
+    calls = [lambda: ops.block_attention(q, k, v, blocks, 16), lambda: ops.block_attention(q[:, :2], k, v, blocks[:, :, :2].contiguous(), 16), lambda: ops.block_scores(q, k),
+             lambda: ops.block_means(k, 16), lambda: ops.select_blocks(ops.block_scores(q, ops.block_means(k, 16)), 3, 16, 70), lambda: ops.embedding(ids, table),
+             lambda: torch.cat([g.flatten() for g in torch.ops.cutespmm.block_attention_grad(dout, q, k, v, out, lse, blocks, 16, None, 0.125)]),
+             lambda: torch.ops.cutespmm.embedding_grad(ids, torch.ones(30, 16, device="cuda"), 50, 1.0)]
+    for fn in calls:
+        want = fn()
+        fn()  # its memory is in torch's cache
+        assert torch.equal(in_a_new_thread(fn), want)
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 

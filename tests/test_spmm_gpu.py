@@ -832,3 +832,30 @@ def test_first_product_on_another_stream_sees_a_finished_plan(oracle_mod):
         p.spmm(B, C, stream=side)
         side.synchronize()
         assert oracle_mod.rel_fro(want, C.cpu().numpy()) <= REL_FRO_TOL_FP32
+
+
+@pytest.mark.parametrize("path", PATHS, ids=["rows", "brick", "auto", "slab"])
+def test_the_first_call_of_a_thread(path):
+    """A worker thread that has asked nothing of the device before: its product may describe B to the driver before any other call."""
+    import threading
+
+    gd = load_golden("elasticity_4")
+    p = cs.Plan(int(gd["M"]), int(gd["K"]), gd["row_ptr"], gd["cols"], gd["vals"], path=path)
+    B = torch.from_numpy(np.ascontiguousarray(gd["B"])).cuda()
+    want, got = torch.full((p.M, B.shape[1]), float("nan"), device="cuda"), torch.full((p.M, B.shape[1]), float("nan"), device="cuda")
+    p.spmm(B, want)
+    torch.cuda.synchronize()
+    failed = []
+
+    def body():
+        try:
+            p.spmm(B, got)
+        except Exception as e:  # noqa: BLE001 -- shown by the thread that waits
+            failed.append(e)
+
+    t = threading.Thread(target=body)
+    t.start()
+    t.join()
+    assert not failed, failed[0]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
