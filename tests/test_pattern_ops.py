@@ -958,6 +958,44 @@ def test_the_first_call_of_a_thread():
         assert torch.equal(in_a_new_thread(fn), want)
 
 
+@pytest.mark.gpu
+def test_compiled():
+    """torch.compile through all of them, forward and backward, is the eager call."""
+    torch.manual_seed(21)
+    tokens = torch.randint(0, 300, (2, 150), device="cuda")
+    table = (torch.randn(300, 96, device="cuda") / 10).bfloat16().requires_grad_(True)
+    weights = [(torch.randn(96, h * 64, device="cuda") / 10).bfloat16().requires_grad_(True) for h in (8, 2, 2)]
+
+    def step(tokens, table, *weights):
+        return layer(tokens, table, *weights, 8, 2, 16, 4)[0]
+
+    want = step(tokens, table, *weights)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(tokens, table, *weights)
+    dout = torch.randn(want.shape, device="cuda").bfloat16()
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, (table, *weights), dout), torch.autograd.grad(want, (table, *weights), dout)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_compiled_single_token_over_pages():
+    """The branch that a decoding program compiles: kept means, a selection, attention over a paged cache."""
+    torch.manual_seed(25)
+    cache = [torch.randn(40, 64, 2, 64, device="cuda").bfloat16() for _ in range(2)]
+    pages, see = torch.randperm(40, device="cuda").view(2, 20).int(), torch.tensor([[1200], [77]], device="cuda", dtype=torch.int32)
+    q = torch.randn(2, 1, 8, 64, device="cuda").bfloat16()
+    means = ops.block_means(cache[0][pages.long()].view(2, 1280, 2, 64), 64, see[:, 0].contiguous())
+
+    def step(q, k, v, means, see, pages):
+        blocks = ops.select_blocks(ops.block_scores(q, means), 5, 64, 1280, see)
+        return blocks, ops.block_attention(q, k, v, blocks, 64, see, None, pages)
+
+    with torch.no_grad():
+        want = step(q, *cache, means, see, pages)
+        got = torch.compile(step, backend="aot_eager", fullgraph=True)(q, *cache, means, see, pages)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ---- calls of the C ABI that the torch operators do not make ---------------------------------------------------------
 
 
