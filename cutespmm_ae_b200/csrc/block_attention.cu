@@ -23,18 +23,19 @@ namespace {
 
 __device__ uint32_t g_status;  // set to 1 when a bounded wait gives up
 
-// A unit of keys in shared memory: DP / 64 tiles of UNIT rows x 128 bytes (swizzled) of keys, then the same of values.
-template <int DP, int UNIT> constexpr int kHalfBytes = DP / 64 * UNIT * 128;
-template <int DP, int UNIT> constexpr int kUnitBytes = 2 * kHalfBytes<DP, UNIT>;
+// A unit of keys of the single-token kernel in shared memory: DP / 64 tiles of 16 rows x 128 bytes (swizzled) of keys, then the same of values.
+constexpr int kSplitUnit = 16;
+template <int DP> constexpr int kHalfBytes = DP / 64 * kSplitUnit * 128;
+template <int DP> constexpr int kUnitBytes = 2 * kHalfBytes<DP>;
 
-template <int DP, int UNIT>
+template <int DP>
 __device__ __forceinline__ void load_unit(unsigned char *stage, const CUtensorMap *k_map, const CUtensorMap *v_map, int kv, int row, int outer, uint64_t *bar)
 {
-    ptx::mbar_expect_tx(bar, kUnitBytes<DP, UNIT>);
+    ptx::mbar_expect_tx(bar, kUnitBytes<DP>);
 #pragma unroll
-    for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + h * UNIT * 128, k_map, h * 64, kv, row, outer, bar);
+    for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + h * kSplitUnit * 128, k_map, h * 64, kv, row, outer, bar);
 #pragma unroll
-    for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + kHalfBytes<DP, UNIT> + h * UNIT * 128, v_map, h * 64, kv, row, outer, bar);
+    for (int h = 0; h < DP / 64; ++h) tc::tma_load4(stage + kHalfBytes<DP> + h * kSplitUnit * 128, v_map, h * 64, kv, row, outer, bar);
 }
 
 // Softmax state and accumulator of one tile of eight columns in the registers of a warp.  A lane holds columns 2 (lane % 4) and
@@ -62,14 +63,9 @@ template <class T, int DP> struct ColumnTile {
         sum[0] = sum[1] = 0.f;
     }
     // scores of a unit -> P^T as operand B of the second product
-    template <int KT> __device__ void softmax(float (&s)[KT][4], uint32_t (&p)[KT][2], float scale_log2)
+    __device__ void softmax(const float (&s)[4], uint32_t (&p)[2], float scale_log2)
     {
-        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
-            m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
-        }
+        float m0 = fmaxf(s[0], s[2]), m1 = fmaxf(s[1], s[3]);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(~0u, m0, x));
@@ -92,15 +88,12 @@ template <class T, int DP> struct ColumnTile {
             top[1] = m1;
         }
         const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;  // nothing visible yet: every exponential is 0
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const float e0 = tc::exp2_fast(fmaf(s[k][0], scale_log2, -b0)), e1 = tc::exp2_fast(fmaf(s[k][1], scale_log2, -b1));
-            const float e2 = tc::exp2_fast(fmaf(s[k][2], scale_log2, -b0)), e3 = tc::exp2_fast(fmaf(s[k][3], scale_log2, -b1));
-            sum[0] += e0 + e2;
-            sum[1] += e1 + e3;
-            p[k][0] = tc::transpose8x8(tc::round2<T>(e0, e1));
-            p[k][1] = tc::transpose8x8(tc::round2<T>(e2, e3));
-        }
+        const float e0 = tc::exp2_fast(fmaf(s[0], scale_log2, -b0)), e1 = tc::exp2_fast(fmaf(s[1], scale_log2, -b1));
+        const float e2 = tc::exp2_fast(fmaf(s[2], scale_log2, -b0)), e3 = tc::exp2_fast(fmaf(s[3], scale_log2, -b1));
+        sum[0] += e0 + e2;
+        sum[1] += e1 + e3;
+        p[0] = tc::transpose8x8(tc::round2<T>(e0, e1));
+        p[1] = tc::transpose8x8(tc::round2<T>(e2, e3));
     }
     __device__ void finish_sum()
     {
@@ -112,15 +105,12 @@ template <class T, int DP> struct ColumnTile {
     }
 };
 
-// Operand A of the first product: rows 16 k of the keys, dims 16 s.
-__device__ __forceinline__ uint32_t keys_at(uint32_t keys, int unit, int k, int s, uint32_t lane)
+// Operand A of the first product: the 16 keys of a unit, dims 16 s.
+__device__ __forceinline__ uint32_t keys_at(uint32_t keys, int s, uint32_t lane) { return keys + (s >> 2) * kSplitUnit * 128 + tc::swizzled(lane & 15, (s & 3) * 2 + (lane >> 4)); }
+// Operand A of the second product, transposed on the way: dims 16 d.
+__device__ __forceinline__ uint32_t values_at(uint32_t values, int d, uint32_t lane)
 {
-    return keys + (s >> 2) * unit * 128 + tc::swizzled(k * 16 + (lane & 15), (s & 3) * 2 + (lane >> 4));
-}
-// Operand A of the second product, transposed on the way: dims 16 d, keys 16 k.
-__device__ __forceinline__ uint32_t values_at(uint32_t values, int unit, int k, int d, uint32_t lane)
-{
-    return values + (d >> 2) * unit * 128 + tc::swizzled(k * 16 + ((lane >> 4) << 3) + (lane & 7), (d & 3) * 2 + ((lane >> 3) & 1));
+    return values + (d >> 2) * kSplitUnit * 128 + tc::swizzled(((lane >> 4) << 3) + (lane & 7), (d & 3) * 2 + ((lane >> 3) & 1));
 }
 
 // ---- a tile of queries -------------------------------------------------------------------------------------------------
@@ -400,7 +390,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) block_attention_kernel(const __
 // order of the warps, first inside a thread block, then over the cluster through distributed shared memory: no scratch, no counters, one
 // launch.  Bound: HBM (the named blocks once) in batches: 64 tokens, 64 heads over 8, 48 blocks of 64 keys of a paged cache 148 us, 5.4 TB/s (one thread block
 // an SM with rings twice as deep: 214 us).  A chain of latencies for one sequence: 8 us.
-constexpr int kSplitWarps = 4, kSplitUnit = 16;
+constexpr int kSplitWarps = 4;
 template <int DP> constexpr int kSplitStages = DP == 128 ? 2 : 4;  // 64 KB of keys and values: three thread blocks share an SM
 constexpr uint32_t kSplitCount = 128;  // most blocks of a query
 
@@ -426,7 +416,7 @@ __device__ __forceinline__ float peer_load(const float *p, uint32_t rank)
 }
 
 template <int DP, int NT> struct SplitSmem {
-    static constexpr int kStage = kUnitBytes<DP, kSplitUnit>;
+    static constexpr int kStage = kUnitBytes<DP>;
     static constexpr int kRings = kSplitWarps * kSplitStages<DP> * kStage;
     static constexpr int kPitch = DP + 4;                                      // floats of a column of a partial result
     static constexpr int kRing = kSplitStages<DP> * kStage;                    // of a warp; its partial result takes the ring's place
@@ -445,7 +435,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x, ranks = gridDim.x;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars) + warp * STAGES;
-    uint32_t *list = reinterpret_cast<uint32_t *>(smem + S::kList), *first_of = list + kSplitCount, *size = first_of + kSplitCount;
+    uint32_t *list = reinterpret_cast<uint32_t *>(smem + S::kList), *first_of = list + kSplitCount;
     const uint32_t t = blockIdx.z % a.queries, b = blockIdx.z / a.queries;
     const uint32_t kv = blockIdx.y / chunks, group = a.heads / a.kv_heads, head0 = blockIdx.y % chunks * (8 * NT), heads = min(8u * NT, group - head0);
     if (lane == 0) {
@@ -474,7 +464,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
     }
     __syncthreads();
     if (counts) list[at] = (uint32_t)mine;
-    (void)size;
     __syncthreads();
 
     const uint32_t per_block = a.block / kSplitUnit, units = total * per_block;
@@ -485,7 +474,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
         const uint32_t n = me + i * walkers;
         int row, outer;
         unit_place(a, b, list[n / per_block], n % per_block * kSplitUnit, row, outer);
-        load_unit<DP, kSplitUnit>(ring + i % STAGES * S::kStage, &k_map, &v_map, (int)kv, row, outer, &full[i % STAGES]);
+        load_unit<DP>(ring + i % STAGES * S::kStage, &k_map, &v_map, (int)kv, row, outer, &full[i % STAGES]);
     };
     if (lane == 0)
         for (uint32_t i = 0; i < mine_units && i < (uint32_t)STAGES; ++i) issue(i);
@@ -505,28 +494,28 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
         }
         const int limit = (int)visible - (int)(list[n / per_block] * a.block + n % per_block * kSplitUnit);
         if (limit > 0) {
-            const uint32_t keys = ptx::smem_u32(ring + s * S::kStage), values = keys + kHalfBytes<DP, kSplitUnit>;
-            float sc[NT][1][4];
+            const uint32_t keys = ptx::smem_u32(ring + s * S::kStage), values = keys + kHalfBytes<DP>;
+            float sc[NT][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) sc[j][0][0] = sc[j][0][1] = sc[j][0][2] = sc[j][0][3] = 0.f;
+            for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 uint32_t f[4];
-                tc::ldmatrix4(f, keys_at(keys, kSplitUnit, 0, d, lane));
+                tc::ldmatrix4(f, keys_at(keys, d, lane));
 #pragma unroll
-                for (int j = 0; j < NT; ++j) tc::mma16<T>(sc[j][0], f, tile[j].q[d][0], tile[j].q[d][1]);
+                for (int j = 0; j < NT; ++j) tc::mma16<T>(sc[j], f, tile[j].q[d][0], tile[j].q[d][1]);
             }
-            uint32_t p[NT][1][2];
+            uint32_t p[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                if ((int)(lane >> 2) >= limit) sc[j][0][0] = sc[j][0][1] = -INFINITY;
-                if ((int)(lane >> 2) + 8 >= limit) sc[j][0][2] = sc[j][0][3] = -INFINITY;
+                if ((int)(lane >> 2) >= limit) sc[j][0] = sc[j][1] = -INFINITY;
+                if ((int)(lane >> 2) + 8 >= limit) sc[j][2] = sc[j][3] = -INFINITY;
                 tile[j].softmax(sc[j], p[j], scale_log2);
             }
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 uint32_t f[4];
-                tc::ldmatrix4_trans(f, values_at(values, kSplitUnit, 0, d, lane));
+                tc::ldmatrix4_trans(f, values_at(values, d, lane));
                 if (limit < kSplitUnit) {
                     const int k = 2 * (int)(lane & 3);
                     f[0] = keep_keys(f[0], k, limit);
@@ -535,7 +524,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) block_attention_split_kernel
                     f[3] = keep_keys(f[3], k + 8, limit);
                 }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) tc::mma16<T>(tile[j].o[d], f, p[j][0][0], p[j][0][1]);
+                for (int j = 0; j < NT; ++j) tc::mma16<T>(tile[j].o[d], f, p[j][0], p[j][1]);
             }
         }
         __syncwarp();

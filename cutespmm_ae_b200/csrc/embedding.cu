@@ -394,9 +394,8 @@ cudaError_t launch_embedding(const EmbeddingArgs &a, int sm_count, cudaStream_t 
 
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t vocab, uint32_t dim) { return GradLayout(count, vocab, dim).total; }
 
-cudaError_t launch_embedding_grad(const EmbeddingArgs &a, void *workspace, int sm_count, cudaStream_t s)
+cudaError_t launch_embedding_grad(const EmbeddingArgs &a, void *workspace, cudaStream_t s)
 {
-    (void)sm_count;
     if (a.vocab == 0 || a.dim == 0) return cudaSuccess;
     const GradLayout l(a.count, a.vocab, a.dim);
     char *w = static_cast<char *>(workspace);

@@ -129,7 +129,7 @@ int cutespmm_embedding_grad(int dtype, const void *dout_dev, uint64_t ld_dout, c
     if ((st = cutespmm_internal_usable_device(&dev, &sms)) != CUTESPMM_OK) return st;
     NvtxRange range("cutespmm: embedding gradient");
     const EmbeddingArgs a{dtype, tokens_dev, token_bytes, count, vocab, dim, scale, dout_dev, ld_dout, dtable_dev, ld_dtable};
-    return launched(launch_embedding_grad(a, workspace_dev, sms, stream_of(stream)), "embedding gradient");
+    return launched(launch_embedding_grad(a, workspace_dev, stream_of(stream)), "embedding gradient");
 }
 
 int cutespmm_block_means(int dtype, const void *k_dev, const int64_t k_strides[3], const int32_t *lengths_dev, uint32_t batch, uint32_t keys, uint32_t kv_heads, uint32_t dim,

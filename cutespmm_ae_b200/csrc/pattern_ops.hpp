@@ -22,7 +22,7 @@ struct EmbeddingArgs {
 };
 cudaError_t launch_embedding(const EmbeddingArgs &a, int sm_count, cudaStream_t s);
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t vocab, uint32_t dim);
-cudaError_t launch_embedding_grad(const EmbeddingArgs &a, void *workspace, int sm_count, cudaStream_t s);
+cudaError_t launch_embedding_grad(const EmbeddingArgs &a, void *workspace, cudaStream_t s);
 
 // ---- block_select.cu ----
 struct MeansArgs {
