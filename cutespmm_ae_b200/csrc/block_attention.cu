@@ -3,8 +3,10 @@
 // Two kernels.  A tile of neighbouring queries shares the blocks that several of them name: block_attention_kernel, on tcgen05.  A single
 // token (or few) has its blocks split over the warps of up to eight thread blocks: block_attention_split_kernel, on mma.sync.
 //
-// Softmax with a running maximum and sum per row, in fp32; P is rounded to the 16-bit type for the second product, the sum is taken before
-// that rounding.  A key that a query does not look at never touches its result, whatever stands there.
+// Softmax with a running maximum and sum per row, in fp32.  P is rounded to the 16-bit type for the second product, because the tensor cores
+// multiply 16-bit values by 16-bit values only (as tf32 the product would run at half the rate and V would have to be widened): half a step
+// per term, u sum p |v| at most beside the u |out| of the result's own rounding; the sum is taken before it.  Against 64 bits out is 2.2e-3 off in
+// bf16 where fp32 throughout is 1.6e-3 (16384 queries, 32 blocks of 64), 2.6e-4 for 2.0e-4 in fp16.  A key that a query does not look at never touches its result, whatever stands there.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -120,9 +122,11 @@ __device__ __forceinline__ uint32_t values_at(uint32_t values, int d, uint32_t l
 // spent a third of a tile's time between them.
 // Rows whose query does not name a tile have P = 0 there.  Multiplying only what is named, on mma.sync with a query's eight heads as the columns of
 // an instruction, was slower for every group, block size and dim tried with the blocks of a selection: 8192 queries, 32 heads, 16 blocks of 64, where
-// 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 407 now; 4096 queries, one head to a group, 16 blocks of 16 302 against 94.
+// 16 neighbouring queries name 241 blocks, 40 of them distinct, 1290 us against 407 (in ncu captures 1183 against 341); 4096 queries, one head to a group, 16 blocks of 16 302 against 94.
 // The maximum is raised only when a score exceeds it by 8 (of the base-2 exponent), so that O is rescaled in tensor memory a few times per row instead of once per
-// tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM: one multiplies while the other's rows are at work.
+// tile; P is then at most 256 and out, a quotient, the same.  Two blocks of threads share an SM while their lists
+// leave room (17 KB each for dims beyond 64, 66 KB below): one multiplies while the other's rows are at work.  Many short blocks a query in a long cache take more --
+// one head to a group, 16 blocks of 16 among 32768 keys: 35 KB -- and then a block has its SM to itself; a tile gets smaller only where its lists would not fit at all.
 // 0 times a value that is no number is not 0: rows of V behind the last visible key are zeroed as they land, and a row whose result is
 // not finite is formed again, key by key, from what its query looks at (exact_row).
 // Measured, forward alone: 8192 queries, 32 heads of dim 128 over 4 heads of keys, 16 blocks of 64: 354 to 410 us (tensor pipe 45 % busy, issue slots 36 %);
@@ -642,7 +646,13 @@ cudaError_t launch_block_attention(const AttentionArgs &a, int sm_count, cudaStr
 {
     if (!a.batch || !a.queries || !a.heads || !a.dim) return cudaSuccess;
     const bool bf16 = a.dtype == CUTESPMM_BF16;
-    // few queries: a thread block per query and head of keys, its blocks split over warps
+    // Few queries: a thread block or a cluster per query and head of keys, its blocks split over warps.  Split / tile in us at 1, 4, 5, 16 and 64 queries a sequence, caches of 32768 keys,
+    // dim 128, neighbours agreeing on most blocks:
+    //   1 sequence, 8 heads of keys, groups of 4, 16 blocks of 64:    8.5 / 19   12 / 40    11 / 42     21 / 56     52 / 61
+    //   8 sequences, groups of 8, 16 blocks of 64:                     14 / 19   35 / 43    43 / 50     76 / 69    219 / 77
+    //   64 sequences, groups of 8, 48 blocks of 64:                  147 / 131  335 / 262  403 / 284  1119 / 361  4315 / 1116
+    // Where each is the better depends on the thread blocks a call makes, not on the queries alone: the limit of 4 is right for single tokens and for eight sequences and more, and gives away
+    // a factor of two to four for 5 to 32 queries of one sequence.
     const bool split = a.queries <= 4;
     const uint32_t rows = a.pages ? a.block : a.keys, outer = a.pages ? a.num_pages : a.batch;
     const uint32_t box = split ? (uint32_t)kSplitUnit : a.pages && a.block < 64 ? a.block : 64u;

@@ -61,7 +61,7 @@ template <class T> __global__ void __launch_bounds__(kMeanWarps * 32) block_mean
 // SM walks jobs of 128 queries x up to 512 means: q comes from memory once, through a ring of TMA tiles, each multiplied with two tiles of 256 means that
 // stay in shared memory (they are the same operand for every head).  Eight warps write the two accumulators out.  With up to 256 means a job uses one
 // accumulator, in turn, and the ring is twice as deep.  Bound: HBM (q and the scores) and the tensor cores about equally (32768 queries, 32 heads, 512 blocks:
-// 82 and 70 us); it takes 131 us, because the write-out of a job with two accumulators is not hidden.  A thread block per 128 x 256 tile, two on an SM: 140 us.
+// 82 and 70 us); it takes 131 us (121 in an ncu capture), because the write-out of a job with two accumulators is not hidden.  A thread block per 128 x 256 tile, two on an SM: 140 us.
 constexpr int kScoreRows = 128, kScoreCols = 256, kScoreMaxStages = 8;
 constexpr int kScoreStageBytes = kScoreRows * 128;
 constexpr int kScoreMeansBytes = 2 * kScoreCols * 128;                       // 256 rows of up to 128 dims

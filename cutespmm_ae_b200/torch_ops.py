@@ -27,8 +27,10 @@ have no counterpart in the reference:
     blocks = select_blocks(scores, count, block, keys)       # the blocks of the highest scores, per query
     out = block_attention(q, k, v, blocks, block)            # attention over those; differentiable with respect to q, k and v
 
-Each is an operator `torch.ops.cutespmm.<name>` as well, runs on torch's current stream of the operands' device, and may be captured
-in a CUDA graph.  Operands whose strides or alignment a kernel cannot read are copied first.
+Each is an operator `torch.ops.cutespmm.<name>` as well (that of `block_attention` also returns the logarithm of each row's sum of exponentials,
+float32 [batch, heads, queries], without a gradient), runs on torch's current stream of the operands' device, and may be captured in a
+CUDA graph.  Operands whose strides or alignment a kernel cannot read are copied first.  Gradients are those of a backward pass; a
+forward-mode derivative is refused.
 """
 from __future__ import annotations
 
