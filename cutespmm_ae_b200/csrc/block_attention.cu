@@ -601,7 +601,8 @@ template <class T, int DP, int NT> cudaError_t launch_split(const CUtensorMap &k
     const uint32_t group = a.heads / a.kv_heads, chunks = (group + 8 * NT - 1) / (8 * NT);
     const uint64_t rows = (uint64_t)a.batch * a.queries * a.kv_heads * chunks, units = (uint64_t)a.count * (a.block / kSplitUnit);
     // thread blocks per query: enough for a few rounds of three on each SM, so that the last round costs little, while a warp has four pieces
-    // of 16 keys (two where the machine would not be full otherwise)
+    // of 16 keys (two where the machine would not be full otherwise).  One / this rule / always eight, us, the launches of a graph, dim 128, 8 heads of keys, blocks of 64: 1 token with
+    // 16 blocks 18 / 7.5 / 7.5, with 48 50 / 12 / 12; 4 tokens 51 / 17 / 17, 16 52 / 54 / 55, 64 152 / 141 / 187
     uint32_t ranks = 1;
     while (ranks < 8 && rows * ranks < 12ull * sm_count && units >= (rows * ranks < (uint64_t)sm_count ? 4ull : 8ull) * ranks * kSplitWarps) ranks *= 2;
     cudaLaunchAttribute attr[2]{};

@@ -428,7 +428,8 @@ cudaError_t launch_select_blocks(const SelectArgs &a, int sm_count, cudaStream_t
     const unsigned heads = a.batch * a.kv_heads;
     auto one = [&](auto kernel) { return launch_overlapped(kernel, dim3((a.queries + 3) / 4, heads), dim3(128), 0, s, a); };
     auto eight = [&](auto kernel) { return launch_overlapped(kernel, dim3(a.queries, heads), dim3(256), 0, s, a); };
-    // eight warps a row where there are too few rows to fill the machine with a warp each, or too many scores for one warp's registers
+    // eight warps a row where there are too few rows to fill the machine with a warp each, or too many scores for one warp's registers.  One warp / eight, us, the
+    // launches of a graph: rows of 1024 scores 256: 9.8 / 5.4, 1000: 10.2 / 11.4, 2400: 13.8 / 21; of 256 scores 8: 4.0 / 4.0, 1000: 4.5 / 9.2, 2400: 5.2 / 16, 65536: 58 / 349
     if (a.blocks <= 1024 && (a.blocks <= 32 || rows > (uint64_t)sm_count * 8)) {
         if (a.blocks <= 32) return one(select_blocks_kernel<1, 1>);
         if (a.blocks <= 64) return one(select_blocks_kernel<2, 1>);
