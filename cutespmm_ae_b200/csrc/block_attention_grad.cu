@@ -8,9 +8,10 @@
 // P is formed again in each of the two from lse; nothing of size queries x keys is stored.
 //
 // Roundings to 16 bits, each half a step u: dS as operand of dq and dk, P as operand of dv (the tensor cores multiply 16-bit values by 16-bit
-// values only), out, which delta is formed from, and the results.  Against 64 bits dq is 2.4e-3 to 3.1e-3 off in bf16 where fp32 throughout is 1.7e-3, of which
-// dS and the result make 2.4e-3 (the roundings one by one, simulated); delta from the rounded out adds 0.05e-3 to 0.15e-3 where keys have a mean in common, for which
-// no copy of out in more bits is kept: it would be as large as out again.  fp16: 3.5e-4 for 2.1e-4.
+// values only), out, which delta is formed from, and the results.  Against 64 bits dq is 2.6e-3 to 3.1e-3 off in bf16 where fp32 throughout is 1.7e-3, dk 2.4e-3.
+// The roundings one by one in 64 bits give exactly that: dS and the result 2.5e-3, delta from an exact out rounded once 2.7e-3 to 3.0e-3, from the forward
+// pass's out, which has P's rounding, 2.8e-3 to 3.1e-3 (dk 2.3e-3, 2.4e-3, 2.4e-3); fp16 3.4e-4 to 4.2e-4 where 2.1e-4.  dS makes most of it and has no other form here; for
+// the rest the forward pass would have to leave a second copy of out, as large as the first, for every step.
 // dS beyond fp16's range is infinite, and what it enters is formed again in fp32 (exact_dq_row, exact_key).
 #include <cuda.h>
 #include <cuda_runtime.h>
